@@ -3,13 +3,13 @@
 // the same steps in Python, of which the launch is 2.9.
 //
 // Functions take their arguments by position (accera_amd/f8.py gives them names); a stream is None, for the device's current one, or a raw hipStream_t.
-// Memory that a call allocates comes back to the caller, who keeps it from being reused too early where the stream was a given one.
 #define PY_SSIZE_T_CLEAN
 #include <Python.h>
 
 #include <ATen/ATen.h>
+#include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
 #include <c10/core/DeviceGuard.h>
-#include <c10/hip/HIPStream.h>
+#include <c10/core/StreamGuard.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
 
@@ -94,23 +94,40 @@ bool flag(PyObject* o)
     return v != 0;
 }
 
-// The one GPU of a call's tensors, made current for the call, and the stream it goes to.
+// The one GPU of a call's tensors and the stream that the call goes to, both made current for the call.
+// What it allocates is memory of that stream: of a given one too, for a block that was freed a moment ago on the caller's current stream may have work
+// pending there, which the given stream does not wait for.  Scratch memory is done with when the stream is, and nothing else uses it.  A result that the caller
+// may also use on the stream that was current (having made it wait) is noted as used there, so that it is not handed on before that one is done either.
 struct Place {
-    c10::OptionalDeviceGuard guard;
+    c10::OptionalDeviceGuard device_guard;
+    c10::OptionalStreamGuard stream_guard;
     c10::Device device;
+    std::optional<c10::Stream> current; // the caller's, where another one was given
     void* stream;
     Place(PyObject* given, const Tensor& first, std::initializer_list<const Tensor*> others) : device(first.device()), stream(nullptr)
     {
         REFUSE_IF(!first.is_cuda(), "tensors must live on the GPU (there is no CPU path)");
         for (const Tensor* t : others) REFUSE_IF(t->defined() && t->device() != device, "tensors must live on one GPU");
-        guard.reset_device(device);
-        if (given == Py_None) stream = c10::hip::getCurrentHIPStream(device.index()).stream();
-        else {
-            stream = PyLong_AsVoidPtr(given);
-            if (!stream && PyErr_Occurred()) throw python_error();
-        }
+        device_guard.reset_device(device);
+        // (torch on ROCm calls the GPU a CUDA device, in its streams too)
+        const auto now = c10::hip::getCurrentHIPStreamMasqueradingAsCUDA(device.index());
+        stream = now.stream();
+        if (given == Py_None) return;
+        void* const other = PyLong_AsVoidPtr(given);
+        if (!other && PyErr_Occurred()) throw python_error();
+        if (other == stream) return;
+        stream = other;
+        current = now.unwrap();
+        stream_guard.reset_stream(other ? c10::hip::getStreamFromExternalMasqueradingAsCUDA((hipStream_t)other, device.index()).unwrap()
+                                        : c10::hip::getDefaultHIPStreamMasqueradingAsCUDA(device.index()).unwrap());
     }
-    Tensor empty(at::IntArrayRef shape, at::ScalarType type) const { return at::empty(shape, at::TensorOptions().dtype(type).device(device)); }
+    Tensor scratch(at::IntArrayRef shape, at::ScalarType type) const { return at::empty(shape, at::TensorOptions().dtype(type).device(device)); }
+    Tensor result(Tensor t) const
+    {
+        if (current) t.record_stream(*current);
+        return t;
+    }
+    Tensor result(at::IntArrayRef shape, at::ScalarType type) const { return result(scratch(shape, type)); }
 };
 
 // an entry point's status as the exception that the rest of the package raises
@@ -127,11 +144,7 @@ void check(int rc)
     throw python_error();
 }
 
-PyObject* wrap(const Tensor& t)
-{
-    if (!t.defined()) Py_RETURN_NONE;
-    return THPVariable_Wrap(t);
-}
+PyObject* wrap(const Tensor& t) { return THPVariable_Wrap(t); }
 PyObject* pair(const Tensor& a, const Tensor& b)
 {
     PyObject *x = wrap(a), *y = wrap(b);
@@ -167,7 +180,7 @@ PyObject* quantize(PyObject* const* a)
     const int64_t groups = (rows + c.group_rows - 1) / c.group_rows, blocks = blocks_of(cols);
     if (!q.defined()) {
         const int64_t pitch = (cols + 15) / 16 * 16; // (rows that the product can fetch 16 bytes at a time)
-        q = place.empty({rows, pitch}, F8);
+        q = place.result({rows, pitch}, F8);
         if (pitch != cols) q = q.narrow(1, 0, cols);
     } else {
         fits(q, {rows, cols}, F8, "out");
@@ -175,7 +188,7 @@ PyObject* quantize(PyObject* const* a)
     }
     if (!scale.defined()) {
         const int64_t strides[2] = {c.group_rows == 1 ? 1 : blocks, c.group_rows == 1 ? groups : 1};
-        scale = at::empty_strided({groups, blocks}, strides, at::TensorOptions().dtype(at::kFloat).device(place.device));
+        scale = place.result(at::empty_strided({groups, blocks}, strides, at::TensorOptions().dtype(at::kFloat).device(place.device)));
     } else fits(scale, {groups, blocks}, at::kFloat, "scale");
     c.x = data(x); c.x_row_stride = x.stride(0); c.x_col_stride = x.stride(1);
     c.q = data(q); c.q_row_stride = q.stride(0);
@@ -185,7 +198,7 @@ PyObject* quantize(PyObject* const* a)
     return pair(q, scale);
 }
 
-// (A, a_scale, B, b_scale, C, epilogue, variant, k_slices, stream) -> scratch memory or None
+// (A, a_scale, B, b_scale, C, epilogue, variant, k_slices, stream)
 PyObject* gemm(PyObject* const* a)
 {
     const Tensor &A = tensor(a[0], "A"), &a_scale = tensor(a[1], "a_scale"), &B = tensor(a[2], "B"), &b_scale = tensor(a[3], "b_scale"), &C = tensor(a[4], "C");
@@ -210,11 +223,11 @@ PyObject* gemm(PyObject* const* a)
     c.C = data(C); c.c_row_stride = C.stride(0); c.c_col_stride = C.stride(1);
     c.workspace_bytes = std::max<int64_t>(acc950_f8_gemm_workspace(&c), 0); // (negative: the call refuses and says why)
     Tensor workspace;
-    if (c.workspace_bytes) workspace = place.empty({c.workspace_bytes}, at::kByte);
+    if (c.workspace_bytes) workspace = place.scratch({c.workspace_bytes}, at::kByte);
     c.workspace = data(workspace);
     c.stream = place.stream;
     check(acc950_f8_gemm(&c));
-    return wrap(workspace);
+    Py_RETURN_NONE;
 }
 
 // (logits, top_k, score, bias, groups, top_groups or None, group_score, renormalise, scale, stream) -> (ids, weights)
@@ -240,7 +253,7 @@ PyObject* route(PyObject* const* a)
         contiguous(bias, "bias");
     }
     const Place place(a[9], logits, {&bias});
-    const Tensor ids = place.empty({c.tokens, c.top_k}, at::kInt), weights = place.empty({c.tokens, c.top_k}, at::kFloat);
+    const Tensor ids = place.result({c.tokens, c.top_k}, at::kInt), weights = place.result({c.tokens, c.top_k}, at::kFloat);
     c.logits = data(logits); c.l_row_stride = logits.stride(0);
     c.bias = data(bias); c.ids = data(ids); c.weights = data(weights);
     c.stream = place.stream;
@@ -266,7 +279,7 @@ PyObject* route_backward(PyObject* const* a)
     c.renormalise = flag(a[4]);
     c.route_scale = real(a[5]);
     const Place place(a[7], logits, {&ids, &dweights, &out});
-    if (!out.defined()) out = place.empty({c.tokens, c.experts}, logits.scalar_type());
+    if (!out.defined()) out = place.result({c.tokens, c.experts}, logits.scalar_type());
     else {
         fits(out, {c.tokens, c.experts}, logits.scalar_type(), "out");
         rows_contiguous(out, "out");
@@ -291,7 +304,7 @@ PyObject* plan(PyObject* const* a)
     c.experts = integer(a[1]);
     const Place place(a[2], ids, {});
     const int64_t pairs = c.tokens * c.top_k, need = acc950_expert_plan_workspace(c.tokens, c.top_k, c.experts); // (negative: the call refuses and says why)
-    const Tensor all = place.empty({2 * pairs + std::max<int64_t>(c.experts, 0) + 1 + std::max<int64_t>(need, 0) / 4}, at::kInt);
+    const Tensor all = place.result({2 * pairs + std::max<int64_t>(c.experts, 0) + 1 + std::max<int64_t>(need, 0) / 4}, at::kInt);
     int* at = (int*)data(all);
     c.ids = data(ids); c.order = at; c.position = at + pairs; c.offsets = at + 2 * pairs;
     c.workspace = at + 2 * pairs + std::max<int64_t>(c.experts, 0) + 1;
@@ -353,7 +366,7 @@ PyObject* combine(PyObject* const* a)
         contiguous(weights, "weights");
     }
     const Place place(a[6], x, {&all, &weights, &out});
-    if (!out.defined()) out = place.empty({c.tokens, c.cols}, x.scalar_type());
+    if (!out.defined()) out = place.result({c.tokens, c.cols}, x.scalar_type());
     else fits(out, {c.tokens, c.cols}, x.scalar_type(), "out");
     REFUSE_IF(c.cols > 1 && (x.stride(1) != 1 || out.stride(1) != 1), "x and out must be contiguous along their last axis");
     c.x = data(x); c.x_row_stride = x.stride(0);
@@ -365,7 +378,7 @@ PyObject* combine(PyObject* const* a)
     return wrap(out);
 }
 
-// (x, ids, weights, w13, w13_scale, w2, w2_scale, out, workspace, stream) -> (out, workspace)
+// (x, ids, weights, w13, w13_scale, w2, w2_scale, out, workspace, stream) -> out
 PyObject* expert_ffn(PyObject* const* a)
 {
     const Tensor &x = tensor(a[0], "x"), &ids = tensor(a[1], "ids"), &weights = tensor(a[2], "weights"), &w13 = tensor(a[3], "w13"), &w13_scale = tensor(a[4], "w13_scale"),
@@ -385,11 +398,11 @@ PyObject* expert_ffn(PyObject* const* a)
     REFUSE_IF(!w13.is_contiguous() || !w2.is_contiguous() || !w13_scale.is_contiguous() || !w2_scale.is_contiguous() || !ids.is_contiguous() || !weights.is_contiguous(),
               "weights, their scales, ids and routing weights must be contiguous");
     const Place place(a[9], x, {&ids, &weights, &w13, &w13_scale, &w2, &w2_scale, &out, &workspace});
-    if (!out.defined()) out = place.empty({c.tokens, c.hidden}, x.scalar_type());
+    if (!out.defined()) out = place.result({c.tokens, c.hidden}, x.scalar_type());
     else fits(out, {c.tokens, c.hidden}, x.scalar_type(), "out");
     REFUSE_IF(c.hidden > 1 && (x.stride(1) != 1 || out.stride(1) != 1), "x and out must be contiguous along their last axis");
     const int64_t need = acc950_f8_expert_ffn_workspace(c.tokens, c.hidden, c.inner, c.experts, c.top_k);
-    if (!workspace.defined()) workspace = place.empty({std::max<int64_t>(need, 1)}, at::kByte);
+    if (!workspace.defined()) workspace = place.scratch({std::max<int64_t>(need, 1)}, at::kByte);
     else REFUSE_IF(workspace.scalar_type() != at::kByte || !workspace.is_contiguous() || workspace.numel() < need, "workspace must be a contiguous uint8 tensor of at least ", need,
                    " elements");
     c.x = data(x); c.x_row_stride = x.stride(0);
@@ -399,7 +412,7 @@ PyObject* expert_ffn(PyObject* const* a)
     c.workspace = data(workspace);
     c.stream = place.stream;
     check(acc950_f8_expert_ffn(&c));
-    return pair(out, workspace);
+    return wrap(out);
 }
 
 template <PyObject* (*RUN)(PyObject* const*), int COUNT>

@@ -2,8 +2,9 @@
 e4m3, the block-scaled product, routing to experts and the experts' products.  torch supplies device memory and streams, every
 computation happens in the HIP kernels of libaccera_mi355x.so.
 
-Calls are asynchronous on the current stream of the tensors' device, or on ``stream`` (a raw hipStream_t).  Results that are not
-passed in are allocated; under a graph capture that works as for any torch allocation.
+Calls are asynchronous on the current stream of the tensors' device, or on ``stream`` (a raw hipStream_t), which then has to wait by itself for whatever
+makes the inputs.  Results that are not passed in are allocated, as torch's allocator does it for work on that stream; under a graph capture that works as for
+any torch allocation.
 
 A layer y = x @ W.T, with W (N, K):
 
@@ -56,17 +57,6 @@ def _raw(stream):
     return (stream.value or 0) if isinstance(stream, ctypes.c_void_p) else stream
 
 
-def _used_on(stream, *allocated):
-    """Tensors that were allocated for a call on a stream given by the caller: the allocator must not hand their memory on before that
-    stream is done with it."""
-    for t in allocated:
-        if t is not None:
-            if stream:
-                t.record_stream(torch.cuda.ExternalStream(stream, device=t.device))
-            else:
-                t.record_stream(torch.cuda.default_stream(t.device))
-
-
 def quantize_f8(x, out=None, scale=None, *, group_rows=1, transpose=False, activation="none", power_of_two=False, stream=None):
     """(q, scale): e4m3 values and fp32 block scales of act(x), a matrix of fp32 / fp16 / bf16; q * scale (spread over its blocks) is
     what they stand for.
@@ -82,12 +72,7 @@ def quantize_f8(x, out=None, scale=None, *, group_rows=1, transpose=False, activ
     act = _ACTIVATIONS.get(activation)
     if act is None:
         raise ValueError(f"unknown activation {activation!r}")
-    if stream is None:
-        return _native.quantize(x, out, scale, group_rows, transpose, act, power_of_two, None)
-    stream = _raw(stream)
-    q, s = _native.quantize(x, out, scale, group_rows, transpose, act, power_of_two, stream)
-    _used_on(stream, *([q] if out is None else []), *([s] if scale is None else []))
-    return q, s
+    return _native.quantize(x, out, scale, group_rows, transpose, act, power_of_two, _raw(stream))
 
 
 def gemm_f8(A, a_scale, B, b_scale, C, epilogue=_lib.EPILOGUE_NONE, variant=_lib.VARIANT_AUTO, k_slices=0, stream=None):
@@ -99,11 +84,7 @@ def gemm_f8(A, a_scale, B, b_scale, C, epilogue=_lib.EPILOGUE_NONE, variant=_lib
     contiguous along K, with rows on 16-byte boundaries (as quantize_f8 leaves them), are taken as they lie, others laid out anew first.  A small result with a long sum is computed in slices
     of K, added in a fixed order; ``variant`` and ``k_slices`` name a kernel and a number of slices (of a tile kernel) instead.
     """
-    if stream is None:
-        _native.gemm(A, a_scale, B, b_scale, C, epilogue, variant, k_slices, None)
-    else:
-        stream = _raw(stream)
-        _used_on(stream, _native.gemm(A, a_scale, B, b_scale, C, epilogue, variant, k_slices, stream))
+    _native.gemm(A, a_scale, B, b_scale, C, epilogue, variant, k_slices, _raw(stream))
     return C
 
 
@@ -122,12 +103,7 @@ def route_experts(logits, top_k, *, score="softmax", bias=None, groups=1, top_gr
     of_group = code if group_score is None else _GROUP_SCORES.get(group_score)
     if of_group is None:
         raise ValueError(f"unknown group_score {group_score!r}")
-    if stream is None:
-        return _native.route(logits, top_k, code, bias, groups, top_groups, of_group, renormalise, scale, None)
-    stream = _raw(stream)
-    ids, weights = _native.route(logits, top_k, code, bias, groups, top_groups, of_group, renormalise, scale, stream)
-    _used_on(stream, ids, weights)
-    return ids, weights
+    return _native.route(logits, top_k, code, bias, groups, top_groups, of_group, renormalise, scale, _raw(stream))
 
 
 def route_experts_backward(logits, ids, dweights, *, score="softmax", renormalise=True, scale=1.0, out=None, stream=None):
@@ -135,13 +111,7 @@ def route_experts_backward(logits, ids, dweights, *, score="softmax", renormalis
     code = _SCORES.get(score)
     if code is None:
         raise ValueError(f"unknown score {score!r}")
-    if stream is None:
-        return _native.route_backward(logits, ids, dweights, code, renormalise, scale, out, None)
-    stream = _raw(stream)
-    grad = _native.route_backward(logits, ids, dweights, code, renormalise, scale, out, stream)
-    if out is None:
-        _used_on(stream, grad)
-    return grad
+    return _native.route_backward(logits, ids, dweights, code, renormalise, scale, out, _raw(stream))
 
 
 class ExpertPlan:
@@ -161,12 +131,7 @@ class ExpertPlan:
 
 def plan_experts(ids, experts, stream=None):
     """The ExpertPlan of ids (tokens, top_k) int32; a number outside 0 .. experts - 1 means no expert, and its pair comes last."""
-    if stream is not None:
-        stream = _raw(stream)
-    plan = ExpertPlan(ids.shape[0], ids.shape[-1], experts, _native.plan(ids, experts, stream))
-    if stream is not None:
-        _used_on(stream, plan._all)
-    return plan
+    return ExpertPlan(ids.shape[0], ids.shape[-1], experts, _native.plan(ids, experts, _raw(stream)))
 
 
 def expert_gemm_f8(A, a_scale, B, b_scale, plan, C, *, gather, row_weights=None, variant=_lib.VARIANT_AUTO, stream=None):
@@ -182,11 +147,7 @@ def expert_gemm_f8(A, a_scale, B, b_scale, plan, C, *, gather, row_weights=None,
 
 def combine_experts(x, plan, weights=None, out=None, stream=None):
     """y[t] = sum over t's slots of weights[t, slot] * x[plan.position[t, slot]] (weights None: of 1), fp32 sums, in x's type."""
-    stream = _raw(stream)
-    y = _native.combine(x, plan._all, plan.tokens, plan.top_k, weights, out, stream)
-    if stream is not None and out is None:
-        _used_on(stream, y)
-    return y
+    return _native.combine(x, plan._all, plan.tokens, plan.top_k, weights, out, _raw(stream))
 
 
 def expert_ffn_f8(x, ids, weights, w13, w13_scale, w2, w2_scale, out=None, workspace=None, stream=None):
@@ -197,11 +158,7 @@ def expert_ffn_f8(x, ids, weights, w13, w13_scale, w2, w2_scale, out=None, works
     are rounded once, to their codes; all sums are fp32.  ``workspace``: a uint8 tensor of
     at least expert_ffn_workspace(...) bytes to be used over and over, or None to allocate one.
     """
-    stream = _raw(stream)
-    y, scratch = _native.expert_ffn(x, ids, weights, w13, w13_scale, w2, w2_scale, out, workspace, stream)
-    if stream is not None:
-        _used_on(stream, *([y] if out is None else []), *([scratch] if workspace is None else []))
-    return y
+    return _native.expert_ffn(x, ids, weights, w13, w13_scale, w2, w2_scale, out, workspace, _raw(stream))
 
 
 def expert_ffn_workspace(tokens, hidden, inner, experts, top_k):
