@@ -97,6 +97,16 @@ __device__ __forceinline__ double key_of(float v, int at)
 __device__ __forceinline__ int index_of_key(double d) { return high_word(d) < 0 ? __double2loint(d) & (MAX_EXPERTS - 1) : MAX_EXPERTS - 1 - (__double2loint(d) & (MAX_EXPERTS - 1)); }
 __device__ __forceinline__ float value_of_key(double d) { return high_word(d) == NAN_KEY ? NAN : (float)d; } // (what lies below a float's last place rounds away)
 
+// A group's key from its two best: their fp32 sum, or where that passes fp32's range (the type's lowest number as a mask, twice) their sum as a double, its last
+// bits cleared for the group's number.  (An infinity below would lie under "nothing to choose", and with the number in its low bits be a NaN.)
+__device__ __forceinline__ double key_of_sum(float best, float second, int at)
+{
+    const float sum = best + second;
+    const double wide = (double)best + (double)second;
+    if (fabsf(sum) < INFINITY || !(fabs(wide) < (double)INFINITY)) return key_of(sum, at);
+    return __hiloint2double(__double2hiint(wide), (__double2loint(wide) & -MAX_EXPERTS) | (wide < 0 ? at : MAX_EXPERTS - 1 - at));
+}
+
 // over the L lanes of a token, the result in all of them: turns within rows of 16 lanes, then the four rows' by scalar registers
 template <int L, typename T, typename Op>
 __device__ __forceinline__ T over_lanes(T v, Op&& op)
@@ -214,7 +224,7 @@ __global__ void __launch_bounds__(256) route_kernel(RouteArgs a, int per, int la
             if (two) second = larger(larger(second, __shfl_xor(second, d)), smaller(best, other));
             best = larger(best, other);
         }
-        if (two && high_word(best) != NO_KEY) best = key_of(value_of_key(best) + (high_word(second) != NO_KEY ? value_of_key(second) : 0.f), group);
+        if (two && high_word(best) != NO_KEY) best = key_of_sum(value_of_key(best), high_word(second) != NO_KEY ? value_of_key(second) : 0.f, group);
         bool open = false;
         for (int n = 0; n < a.top_groups; ++n) {
             const double taken = over_lanes<L>(best, larger);

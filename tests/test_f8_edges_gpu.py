@@ -1,7 +1,8 @@
 """Feed-forward operators in 8-bit floating point at the edges of their ranges: streams, masks and values as large or as small as their types allow."""
+import numpy as np
 import pytest
 
-from test_f8_gpu import _codes, _rand, _scales, acc  # noqa: F401
+from test_f8_gpu import U, _apart, _codes, _rand, _route64, _scales, acc  # noqa: F401
 
 pytestmark = pytest.mark.gpu
 
@@ -79,3 +80,50 @@ def test_streams_by_number(acc):  # noqa: F811
         side.wait_stream(torch.cuda.default_stream())
         assert torch.equal(q.float(), want)
         assert torch.cuda.current_stream() == side
+
+
+# ---- routing -----------------------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("tokens", [3, 5000])
+@pytest.mark.parametrize("experts,groups,k", [(64, 8, 6), (64, 8, 16), (64, 4, 40), (256, 8, 8), (1024, 64, 32), (60, 3, 5), (16, 16, 3)])
+def test_route_masks_of_the_lowest_number(acc, experts, groups, k, tokens):  # noqa: F811
+    """A bias of fp32's lowest number on whole groups and inside them, as a mask has it: such experts come last, and are still experts where no others are left (the
+    sum of two such scores lies below every fp32 number).  The same at the other end, where a bias of the largest opens groups."""
+    import torch
+    per, low = experts // groups, float(np.finfo(np.float32).min)
+    rng = np.random.default_rng(experts + k)
+    x = _apart(experts, tokens, experts, gap=0.2)
+    masks = [[0], [groups - 1], [1], list(range(groups - 1)), list(range(1, groups)), list(range(groups)), list(range(0, groups, 2))]
+    for group_score in ("best_two", "best"):
+        for n, mask in enumerate(masks):
+            for value in (low, low / 2, -low):
+                bias = (np.arange(experts) % (5 if experts <= 256 else 1) * 2.0 ** -12).astype(np.float32)
+                for g in mask:
+                    bias[g * per:(g + 1) * per] = value
+                if n == 1 and per > 2:
+                    bias[1], bias[per + 1:per + per] = value, value  # (one of a group's experts, all but one of another's)
+                if n == 2:
+                    bias[per:2 * per][rng.random(per) < 0.3] = -np.inf
+                for top in sorted({1, (groups + 1) // 2, groups}):
+                    some = x[:40]
+                    want_ids, want = _route64(some, k, "sigmoid", bias, groups, top, group_score, True, 1.0)
+                    ids, w = acc.route_experts(torch.from_numpy(x).cuda(), k, score="sigmoid", bias=torch.from_numpy(bias).cuda(), groups=groups, top_groups=top, group_score=group_score)
+                    # (scores that a large bias swallows are all the same, in fp32 as in 64 bits: the lowest experts of the lowest groups)
+                    sure = _sure_of(some, bias, groups, top, k, group_score)
+                    assert sure.any() or not np.isfinite(bias).any()
+                    assert np.array_equal(ids[:40].cpu().numpy()[sure], want_ids[sure]), (group_score, mask, value, top)
+                    np.testing.assert_allclose(w[:40].cpu().numpy()[sure], want[sure], rtol=96 * U)
+
+
+def _sure_of(x, bias, groups, top, k, group_score):
+    """Rows whose choice does not hang on a rounding of fp32: no two different values within 2^-20 of each other among the groups' scores or the choices, in their own size."""
+    with np.errstate(over="ignore", invalid="ignore"):
+        p = 1 / (1 + np.exp(-x.astype(np.float64))) + bias.astype(np.float64)
+        both = np.sort(p.reshape(len(x), groups, -1), axis=2)[:, :, ::-1]
+        g = both[:, :, 0] + (np.where(np.isfinite(both[:, :, 1]), both[:, :, 1], 0) if group_score == "best_two" and both.shape[2] > 1 else 0)
+        sure = np.ones(len(x), bool)
+        for v in (p,) if groups == 1 else (p, g):
+            s = np.sort(v, axis=1)
+            gap, size = np.diff(s, axis=1), np.maximum(1.0, np.minimum(np.abs(s[:, 1:]), np.abs(s[:, :-1])))
+            sure &= ~((gap > 0) & (gap < 2.0 ** -20 * size)).any(axis=1)
+    return sure
