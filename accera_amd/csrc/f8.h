@@ -224,13 +224,14 @@ __device__ __forceinline__ unsigned f8_pack4(float a, float b, float c, float d)
 
 // gate / (1 + exp(-gate)) * up, within 8 * 2^-24: exp(-gate) = 2^t * (1 + rest ln 2), t + rest = -gate log2(e) (the product's own rounding goes
 // into `rest`), and the hardware's reciprocal, within one unit.  (With expf and a division the quantiser was bound by its arithmetic:
-// 8192 x 11008 in 148 us.)  Where 2^t is infinite the quotient is 0.
+// 8192 x 11008 in 148 us.)  Where 2^t is infinite the quotient is 0, and below 2^-128 it adds nothing to 1; `rest` is left out of both, for where t itself is
+// infinite (gates past 2.4e38) so is `rest`.
 __device__ __forceinline__ float silu_mul(float gate, float up)
 {
     const float t = gate * -1.44269502f;
     const float rest = fmaf(gate, -1.44269502f, -t) + gate * -1.92596303e-8f;
     const float e = __builtin_amdgcn_exp2f(t);
-    return gate * __builtin_amdgcn_rcpf(1.f + (e < INFINITY ? fmaf(e, rest * 0.693147182f, e) : e)) * up;
+    return gate * __builtin_amdgcn_rcpf(1.f + (fabsf(t) < 128.f ? fmaf(e, rest * 0.693147182f, e) : e)) * up;
 }
 
 // The same for values that become codes at once, half the instructions: the exponent's own rounding moves exp(-gate) by |gate| * 2^-24 of itself, no more than

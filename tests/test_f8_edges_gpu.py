@@ -2,7 +2,7 @@
 import numpy as np
 import pytest
 
-from test_f8_gpu import U, _apart, _codes, _rand, _route64, _scales, acc  # noqa: F401
+from test_f8_gpu import U, _apart, _codes, _dtype, _rand, _route64, _scales, _spread, acc  # noqa: F401
 
 pytestmark = pytest.mark.gpu
 
@@ -127,3 +127,39 @@ def _sure_of(x, bias, groups, top, k, group_score):
             gap, size = np.diff(s, axis=1), np.maximum(1.0, np.minimum(np.abs(s[:, 1:]), np.abs(s[:, :-1])))
             sure &= ~((gap > 0) & (gap < 2.0 ** -20 * size)).any(axis=1)
     return sure
+
+
+# ---- quantising --------------------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+def test_quantise_behind_a_gate_as_large_as_its_type(acc, kind):  # noqa: F811
+    """silu(gate) * up where gate * log2(e) passes fp32's largest number: still gate * up, and 0 on the other side."""
+    import torch
+    gate = torch.tensor([2.3e38, 2.4e38, 2.5e38, 3e38, 3.38e38, -2.4e38, -3e38, -3.38e38, 100.0, -100.0, 88.5, -88.5, 89.0, -89.0, 0.0, 1e30, -1e30], dtype=torch.float32)
+    gate = gate.to(_dtype(kind)).repeat(8)[:128]
+    up = torch.full((128,), 1e-3).to(gate.dtype)
+    for order in range(3):
+        rows = torch.stack([torch.cat([gate.roll(order), up]), torch.cat([gate.roll(order).clamp(-1e3, 1e3), up])])
+        for pow2 in (False, True):
+            q, s = acc.quantize_f8(rows.cuda(), activation="silu_mul", power_of_two=pow2)
+            v = torch.nn.functional.silu(rows[:, :128].double()) * rows[:, 128:].double()
+            full = _spread(s.cpu().double(), 2, 128, 1)
+            step = torch.maximum(v.abs() * 2.0 ** -4, full * 2.0 ** -10)
+            got = q.cpu().double() * full
+            assert torch.isfinite(got).all() and ((got - v).abs() <= step * (1 + 32 * U) + 16 * U * v.abs()).all()
+
+
+def test_quantise_behind_infinite_and_missing_gates(acc):  # noqa: F811
+    """An infinite gate gives an infinite or undefined value, which makes its group NaN, like a NaN on either side; other groups are as they were."""
+    import torch
+    rows = _rand(1, 8, 2 * 256)
+    want = acc.quantize_f8(rows.cuda(), activation="silu_mul")
+    want = (want[0].float() * want[1].repeat_interleave(128, dim=1)).cpu()
+    for at, value in ((5, float("inf")), (6, float("-inf")), (7, float("nan")), (256 + 9, float("nan")), (256 + 10, float("inf"))):
+        bad = rows.clone()
+        bad[3, at] = value
+        q, s = acc.quantize_f8(bad.cuda(), activation="silu_mul")
+        got = (q.float() * s.repeat_interleave(128, dim=1)).cpu()
+        assert torch.isnan(got[3, :128]).all()
+        got[3, :128] = want[3, :128]
+        assert torch.equal(got, want)
