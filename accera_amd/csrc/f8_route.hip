@@ -269,7 +269,8 @@ __global__ void __launch_bounds__(256) route_kernel(RouteArgs a, int per, int la
 
 // 8192x128 in bf16 6.2 us (4.7 MB), 16384x256 14 us: the exponentials of all experts, to the last place as going forward.
 // dlogits.  With g the gradient of the scores taken (g_s = scale * dw_s, or renormalised scale * (dw_s - sum dw w') / total, w' = p / total):
-// sigmoid: p (1 - p) g for the experts taken; softmax: p (g - sum over the taken of p g), g 0 for the others.
+// sigmoid: p (1 - p) g for the experts taken, 1 - p being 1 / (1 + exp(x)), for the difference would have lost its bits where p is nearly 1; softmax: p (g - sum over the
+// taken of p g), g 0 for the others.
 template <int VPL>
 __global__ void __launch_bounds__(256) route_backward_kernel(RouteArgs a)
 {
@@ -287,11 +288,12 @@ __global__ void __launch_bounds__(256) route_backward_kernel(RouteArgs a)
     const bool have = my_id >= 0 && my_id < a.experts;
     float my_g = have ? a.dweights[token * a.top_k + lane] : 0.f;
     scores_of<VPL>(x, p, a.experts, a.score, lane);
-    float my_p = 0.f; // score of this lane's slot
+    const bool sigmoid = a.score == ACC950_SCORE_SIGMOID;
+    float my_p = 0.f, my_x = 0.f; // score and logit of this lane's slot
 #pragma unroll
     for (int j = 0; j < VPL; ++j) {
-        const float v = __shfl(p[j], my_id & 63);
-        if (have && my_id >> 6 == j) my_p = v;
+        const float v = __shfl(p[j], my_id & 63), logit = __shfl(x[j], my_id & 63);
+        if (have && my_id >> 6 == j) { my_p = v; my_x = logit; }
     }
     if (a.renormalise) {
         const float total = wave_sum(my_p);
@@ -299,7 +301,8 @@ __global__ void __launch_bounds__(256) route_backward_kernel(RouteArgs a)
         my_g = total == 0.f || !have ? 0.f : (my_g - dot / total) / total;
     }
     my_g *= a.scale;
-    const float dot = a.score == ACC950_SCORE_SOFTMAX ? wave_sum(my_p * my_g) : 0.f;
+    const float dot = sigmoid ? 0.f : wave_sum(my_p * my_g);
+    if (sigmoid) my_g = have ? my_p * (1.f / (1.f + expf(my_x))) * my_g : 0.f; // (the logit's gradient, where the others have that of the score)
     for (int s = 0; s < a.top_k; ++s) {
         const int e = __builtin_amdgcn_readlane(have ? my_id : -1, s);
         const float gs = __shfl(my_g, s);
@@ -311,7 +314,7 @@ __global__ void __launch_bounds__(256) route_backward_kernel(RouteArgs a)
     for (int j = 0; j < VPL; ++j) {
         const int e = j * 64 + lane;
         if (e < a.experts)
-            store_out(a.dlogits, a.in_type, token * a.g_rs + e, a.score == ACC950_SCORE_SOFTMAX ? p[j] * (g[j] - dot) : p[j] * (1.f - p[j]) * g[j]);
+            store_out(a.dlogits, a.in_type, token * a.g_rs + e, sigmoid ? g[j] : p[j] * (g[j] - dot));
     }
 }
 

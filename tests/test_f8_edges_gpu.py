@@ -163,3 +163,26 @@ def test_quantise_behind_infinite_and_missing_gates(acc):  # noqa: F811
         assert torch.isnan(got[3, :128]).all()
         got[3, :128] = want[3, :128]
         assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("tokens,experts,k", [(5, 64, 6), (40, 300, 20)])
+@pytest.mark.parametrize("renorm", [True, False])
+def test_route_gradient_of_saturated_sigmoids(acc, tokens, experts, k, renorm):  # noqa: F811
+    """p (1 - p) where p is nearly 1: held to a share of itself, not of p."""
+    import torch
+    rng = np.random.default_rng(experts)
+    x = torch.from_numpy(rng.uniform(-40, 40, (tokens, experts)).astype(np.float32))
+    x[0] = torch.linspace(10, 40, experts)
+    x[1] = torch.linspace(-40, -10, experts)
+    dw = _rand(4, tokens, k)
+    ids, _ = acc.route_experts(x.cuda(), k, score="sigmoid", renormalise=renorm, scale=1.5)
+    got = acc.route_experts_backward(x.cuda(), ids, dw.cuda(), score="sigmoid", renormalise=renorm, scale=1.5).double().cpu()
+    z, at, g = x.double(), ids.cpu().long(), 1.5 * dw.double()
+    p = torch.gather(torch.sigmoid(z), 1, at)
+    slope = p * torch.gather(torch.sigmoid(-z), 1, at)
+    total = p.sum(dim=1, keepdim=True) if renorm else torch.ones(tokens, 1, dtype=torch.float64)
+    dot = (g * p / total).sum(dim=1, keepdim=True) if renorm else 0.0
+    want = torch.zeros(tokens, experts, dtype=torch.float64).scatter_(1, at, slope * (g - dot) / total)
+    # exp within 2 units and four roundings on either side of the product, the dot's sum of up to 64 terms with a score's error each, a division: 160 u of each of its terms
+    size = torch.zeros(tokens, experts, dtype=torch.float64).scatter_(1, at, slope * (g.abs() + (g.abs() * p / total).sum(dim=1, keepdim=True)) / total)
+    assert ((got - want).abs() <= 160 * U * size).all(), float(((got - want).abs() / size.clamp(min=1e-300)).max() / U)
