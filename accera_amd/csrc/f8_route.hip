@@ -77,6 +77,10 @@ __device__ __forceinline__ void scores_of(float (&x)[VPL], float (&p)[VPL], int 
     for (int j = 0; j < VPL; ++j) p[j] = p[j] / sum;
 }
 
+// Scores taken that are this small altogether, which a bias may lead to, have few or no bits left (fp32 ends at 2^-126); renormalised they are then worked out again beside the
+// largest of them: softmax's are exp(x) times something that all share, and so are sigmoid's, to 2^-90 of themselves.
+constexpr float SCORES_LOST = 0x1p-90f;
+
 // ---- the choice -----------------------------------------------------------------------------------
 // L lanes to a token, VPL experts to a lane.  Bound by the instructions: 16384x256 in groups reads 16.8 MB (3.2 us) and takes 15 us, a third of it the
 // sigmoids, exact to the last place (expf, IEEE division), for a choice must not hang on a faster one's rounding.  What is chosen from is kept as doubles: the fp32 value exactly, and in the low bits, which a float leaves
@@ -252,13 +256,18 @@ __global__ void __launch_bounds__(256) route_kernel(RouteArgs a, int per, int la
 #pragma unroll
         for (int j = 0; j < VPL; ++j) key[j] = with_high(key[j], id - e0 == j ? NO_KEY : high_word(key[j]));
     }
-    float w = 0.f;
+    float w = 0.f, mine = -INFINITY; // score and logit of the lane's slot
     if (my_id >= 0) {
-        const float v = load_logit(a.logits, a.in_type, row + my_id);
-        w = a.score == ACC950_SCORE_SIGMOID ? sigmoid(v) : softmax(v);
+        mine = load_logit(a.logits, a.in_type, row + my_id);
+        w = a.score == ACC950_SCORE_SIGMOID ? sigmoid(mine) : softmax(mine);
     }
     if (a.renormalise) {
-        const float total = over_lanes<L>(w, [](float u, float v) { return u + v; });
+        float total = over_lanes<L>(w, [](float u, float v) { return u + v; });
+        if (total < SCORES_LOST) {
+            const float largest = over_lanes<L>(mine, [](float u, float v) { return fmaxf(u, v); });
+            w = largest == -INFINITY ? 0.f : expf(mine - largest);
+            total = over_lanes<L>(w, [](float u, float v) { return u + v; });
+        }
         w = total == 0.f ? 0.f : w / total;
     }
     if (lane < a.top_k) {
@@ -295,14 +304,24 @@ __global__ void __launch_bounds__(256) route_backward_kernel(RouteArgs a)
         const float v = __shfl(p[j], my_id & 63), logit = __shfl(x[j], my_id & 63);
         if (have && my_id >> 6 == j) { my_p = v; my_x = logit; }
     }
+    bool lost = false;
     if (a.renormalise) {
-        const float total = wave_sum(my_p);
-        const float dot = wave_sum(my_g * my_p);
-        my_g = total == 0.f || !have ? 0.f : (my_g - dot / total) / total;
+        float total = wave_sum(my_p);
+        lost = total < SCORES_LOST;
+        if (lost) {
+            const float largest = of_order_bits(wave_max_u(order_bits(have ? my_x : -INFINITY)));
+            my_p = have && largest > -INFINITY ? expf(my_x - largest) : 0.f;
+            total = wave_sum(my_p);
+        }
+        const float shares = wave_sum(my_g * my_p);
+        my_g = total == 0.f || !have ? 0.f : (my_g - shares / total) / total;
     }
     my_g *= a.scale;
-    const float dot = sigmoid ? 0.f : wave_sum(my_p * my_g);
-    if (sigmoid) my_g = have ? my_p * (1.f / (1.f + expf(my_x))) * my_g : 0.f; // (the logit's gradient, where the others have that of the score)
+    float dot = 0.f;
+    const bool of_logits = sigmoid || lost; // my_g becomes the gradient of the slot's logit (and is that of its score otherwise)
+    if (lost) my_g *= my_p; // (either score's: softmax's other term, the sum of these, is 0, and 1 - p is 1)
+    else if (sigmoid) my_g = have ? my_p * (1.f / (1.f + expf(my_x))) * my_g : 0.f;
+    else dot = wave_sum(my_p * my_g);
     for (int s = 0; s < a.top_k; ++s) {
         const int e = __builtin_amdgcn_readlane(have ? my_id : -1, s);
         const float gs = __shfl(my_g, s);
@@ -314,7 +333,7 @@ __global__ void __launch_bounds__(256) route_backward_kernel(RouteArgs a)
     for (int j = 0; j < VPL; ++j) {
         const int e = j * 64 + lane;
         if (e < a.experts)
-            store_out(a.dlogits, a.in_type, token * a.g_rs + e, sigmoid ? g[j] : p[j] * (g[j] - dot));
+            store_out(a.dlogits, a.in_type, token * a.g_rs + e, of_logits ? g[j] : p[j] * (g[j] - dot));
     }
 }
 

@@ -98,7 +98,7 @@ int64_t acc950_f8_gemm_workspace(const acc950_f8_gemm_call* call); /* (reads no 
  * Routing: p = softmax or sigmoid of a token's logits (F32 / F16 / BF16, tokens x experts), choice = p + bias (bias: fp32 per
  * expert, or NULL).  Of `groups` equal groups of neighbouring experts the top_groups with the best scores stay open; the top_k best
  * choices of their experts are taken, best first, ties to the lowest number.  weights = route_scale * p, with `renormalise` of
- * p / (sum of the p taken).  ids (int32) and weights (fp32) are tokens x top_k, contiguous.
+ * p / (sum of the p taken), also where these are too small for fp32.  ids (int32) and weights (fp32) are tokens x top_k, contiguous.
  * An expert whose logit or bias is -infinity is never taken; where too few are left, the last ids are -1 and their weights 0.
  * NaN ranks above everything (and its weight is NaN).  Up to 1024 experts, top_k up to 64.
  * acc950_route_backward: gradient of the logits (their type, contiguous rows grad_row_stride apart) from the gradient of the

@@ -186,3 +186,44 @@ def test_route_gradient_of_saturated_sigmoids(acc, tokens, experts, k, renorm): 
     # exp within 2 units and four roundings on either side of the product, the dot's sum of up to 64 terms with a score's error each, a division: 160 u of each of its terms
     size = torch.zeros(tokens, experts, dtype=torch.float64).scatter_(1, at, slope * (g.abs() + (g.abs() * p / total).sum(dim=1, keepdim=True)) / total)
     assert ((got - want).abs() <= 160 * U * size).all(), float(((got - want).abs() / size.clamp(min=1e-300)).max() / U)
+
+
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("tokens,k", [(6, 4), (5000, 20)])
+def test_route_scores_below_the_smallest_number(acc, score, tokens, k):  # noqa: F811
+    """Chosen experts whose scores all vanish beside fp32's smallest number (a bias sets the likely ones aside): their renormalised weights are still those of the formula, and so
+    is the gradient."""
+    import torch
+    experts = 64
+    x = _apart(3, tokens, experts, gap=0.1)
+    x -= 110.0 if score == "sigmoid" else 0.0
+    x[1::2] -= 300.0 if score == "sigmoid" else 0.0
+    bias = np.zeros(experts, np.float32)
+    if score == "softmax":
+        x[:, :8] += 120.0
+        x[1::2, :8] += 300.0
+        bias[:8] = -4.0
+    some = slice(0, 6)
+    ids, w = acc.route_experts(torch.from_numpy(x).cuda(), k, score=score, bias=torch.from_numpy(bias).cuda(), scale=1.5)
+    at = ids[some].cpu().long()
+    if score == "softmax":
+        assert (at >= 8).all()
+    z = torch.from_numpy(x[some]).double()
+    p = torch.gather(torch.sigmoid(z) if score == "sigmoid" else torch.softmax(z, dim=1), 1, at)
+    want = 1.5 * p / p.sum(dim=1, keepdim=True)
+    np.testing.assert_allclose(w[some].cpu().numpy(), want.numpy(), rtol=96 * U)
+    dw = _rand(2, tokens, k)
+    grad = acc.route_experts_backward(torch.from_numpy(x).cuda(), ids, dw.cuda(), score=score, scale=1.5)[some]
+    # the gradient's formula (the experts that are not taken have none; 1 - p is 1 to 64 bits, or softmax's other term 0)
+    g64, dots = dw[some].double(), (want * dw[some].double()).sum(dim=1, keepdim=True) / 1.5
+    g = torch.zeros(z.shape, dtype=torch.float64).scatter_(1, at, want * (g64 - dots))
+    size = torch.zeros_like(g).scatter_(1, at, want * (g64.abs() + (want * g64.abs()).sum(dim=1, keepdim=True)))
+    assert ((grad.double().cpu() - g).abs() <= 160 * U * size).all()
+    if tokens == 6:  # (and differences of the formula)
+        step, direction = 1e-4, _rand(8, 6, experts).double()
+
+        def value(y):
+            e = torch.exp(torch.gather(y, 1, at) - torch.gather(y, 1, at).max(dim=1, keepdim=True)[0])
+            return (1.5 * e / e.sum(dim=1, keepdim=True) * g64).sum()
+        slope = float(value(z + step * direction) - value(z - step * direction)) / (2 * step)
+        assert abs(float((grad.double().cpu() * direction).sum()) - slope) <= 1e-5 * float((size * direction.abs()).sum())
