@@ -6,6 +6,9 @@ Calls are asynchronous on the current stream of the tensors' device, or on ``str
 makes the inputs.  Results that are not passed in are allocated, as torch's allocator does it for work on that stream; under a graph capture that works as for
 any torch allocation.
 
+None of them has a gradient by itself (feed_forward.f8_linear and f8_route do).  Where an input of a routed layer, a weighted sum or a choice asks for one, the
+result carries a node that refuses it.
+
 A layer y = x @ W.T, with W (N, K):
 
     wq, ws = quantize_f8(W, group_rows=128)                 # once
@@ -57,6 +60,26 @@ def _raw(stream):
     return (stream.value or 0) if isinstance(stream, ctypes.c_void_p) else stream
 
 
+class _Refused(torch.autograd.Function):
+    """A result as it is, whose gradient is an error: without this, autograd would take what made it for a constant."""
+
+    @staticmethod
+    def forward(ctx, name, y, *inputs):
+        ctx.name = name
+        return y.view_as(y)
+
+    @staticmethod
+    def backward(ctx, dy):
+        raise RuntimeError(f"{ctx.name} has no gradient: call it under torch.no_grad(), or with inputs that are detached")
+
+
+def without_gradient(name, y, *inputs):
+    """y, the result of ``name`` for these inputs, with a gradient that is refused if any of them asks for one."""
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in inputs):
+        return _Refused.apply(name, y, *inputs)
+    return y
+
+
 def quantize_f8(x, out=None, scale=None, *, group_rows=1, transpose=False, activation="none", power_of_two=False, stream=None):
     """(q, scale): e4m3 values and fp32 block scales of act(x), a matrix of fp32 / fp16 / bf16; q * scale (spread over its blocks) is
     what they stand for.
@@ -103,7 +126,8 @@ def route_experts(logits, top_k, *, score="softmax", bias=None, groups=1, top_gr
     of_group = code if group_score is None else _GROUP_SCORES.get(group_score)
     if of_group is None:
         raise ValueError(f"unknown group_score {group_score!r}")
-    return _native.route(logits, top_k, code, bias, groups, top_groups, of_group, renormalise, scale, _raw(stream))
+    ids, weights = _native.route(logits, top_k, code, bias, groups, top_groups, of_group, renormalise, scale, _raw(stream))
+    return ids, without_gradient("route_experts", weights, logits) if logits.requires_grad else weights
 
 
 def route_experts_backward(logits, ids, dweights, *, score="softmax", renormalise=True, scale=1.0, out=None, stream=None):
@@ -147,7 +171,7 @@ def expert_gemm_f8(A, a_scale, B, b_scale, plan, C, *, gather, row_weights=None,
 
 def combine_experts(x, plan, weights=None, out=None, stream=None):
     """y[t] = sum over t's slots of weights[t, slot] * x[plan.position[t, slot]] (weights None: of 1), fp32 sums, in x's type."""
-    return _native.combine(x, plan._all, plan.tokens, plan.top_k, weights, out, _raw(stream))
+    return without_gradient("combine_experts", _native.combine(x, plan._all, plan.tokens, plan.top_k, weights, out, _raw(stream)), x, weights)
 
 
 def expert_ffn_f8(x, ids, weights, w13, w13_scale, w2, w2_scale, out=None, workspace=None, stream=None):
@@ -158,7 +182,8 @@ def expert_ffn_f8(x, ids, weights, w13, w13_scale, w2, w2_scale, out=None, works
     are rounded once, to their codes; all sums are fp32.  ``workspace``: a uint8 tensor of
     at least expert_ffn_workspace(...) bytes to be used over and over, or None to allocate one.
     """
-    return _native.expert_ffn(x, ids, weights, w13, w13_scale, w2, w2_scale, out, workspace, _raw(stream))
+    y = _native.expert_ffn(x, ids, weights, w13, w13_scale, w2, w2_scale, out, workspace, _raw(stream))
+    return without_gradient("expert_ffn_f8", y, x, weights) if x.requires_grad or weights.requires_grad else y
 
 
 def expert_ffn_workspace(tokens, hidden, inner, experts, top_k):

@@ -17,7 +17,7 @@ import argparse
 import torch
 
 from . import _lib
-from .f8 import BLOCK, F8, expert_ffn_f8, gemm_f8, quantize_f8, route_experts, route_experts_backward
+from .f8 import BLOCK, F8, expert_ffn_f8, gemm_f8, quantize_f8, route_experts, route_experts_backward, without_gradient
 from .gemm import gemm_relu
 
 
@@ -25,7 +25,7 @@ class ExpertLayer:
     """A routed feed-forward layer with weights in e4m3: out[t] = sum over t's experts of weight * down(silu(gate(x[t])) * up(x[t])).
 
     router (hidden, experts) fp16 / bf16; gate, up (experts, inner, hidden) and down (experts, hidden, inner) fp32 / fp16 / bf16, quantised here in blocks
-    of 128 x 128.  ``route``: further arguments of route_experts.
+    of 128 x 128.  ``route``: further arguments of route_experts.  For serving: it has no gradient, and says so where one is asked for.
     """
 
     def __init__(self, router, gate, up, down, top_k, **route):
@@ -47,11 +47,14 @@ class ExpertLayer:
         """(ids, weights) of the experts of x (tokens, hidden), in the router's type; fp32 scores."""
         logits = x.new_empty((x.shape[0], self.router.shape[1]), dtype=torch.float32)
         gemm_relu(x, self.router, logits, epilogue=_lib.EPILOGUE_NONE)
-        return route_experts(logits, self.top_k, **self.route)
+        ids, weights = route_experts(logits, self.top_k, **self.route)
+        return ids, without_gradient("ExpertLayer", weights, x, self.router)
 
     def __call__(self, x, out=None):
-        ids, weights = self.choose(x)
-        return expert_ffn_f8(x, ids, weights, self.w13, self.w13_scale, self.w2, self.w2_scale, out=out)
+        with torch.no_grad():
+            ids, weights = self.choose(x)
+            y = expert_ffn_f8(x, ids, weights, self.w13, self.w13_scale, self.w2, self.w2_scale, out=out)
+        return without_gradient("ExpertLayer", y, x, self.router)
 
 
 class _Linear(torch.autograd.Function):
@@ -70,16 +73,18 @@ class _Linear(torch.autograd.Function):
             dyq, dys = quantize_f8(dy)
             wq, ws = quantize_f8(w, group_rows=BLOCK, transpose=True)
             dx = gemm_f8(dyq, dys, wq.t(), ws.t(), torch.empty_like(x, memory_format=torch.contiguous_format))
+            dx = without_gradient("the gradient of f8_linear", dx, dy, x, w)  # (in a backward pass that is to be differentiated itself)
         if ctx.needs_input_grad[1]:
             # (groups run along the tokens that are summed over; the sum over a batch stays in fp32 until it is the weight's type)
             dyq, dys = quantize_f8(dy, transpose=True)
             xq, xs = quantize_f8(x, transpose=True)
             dw = gemm_f8(dyq, dys, xq.t(), xs.t(), w.new_empty(w.shape, dtype=torch.float32)).to(w.dtype)
+            dw = without_gradient("the gradient of f8_linear", dw, dy, x, w)
         return dx, dw
 
 
 def f8_linear(x, w):
-    """x (tokens, in) @ w (out, in).T in x's type, operands of this product and of both gradients' in e4m3."""
+    """x (tokens, in) @ w (out, in).T in x's type, operands of this product and of both gradients' in e4m3 (once: the gradients have none of their own)."""
     return _Linear.apply(x, w)
 
 
@@ -95,7 +100,8 @@ class _Route(torch.autograd.Function):
     @staticmethod
     def backward(ctx, _, dweights):
         logits, ids = ctx.saved_tensors
-        return route_experts_backward(logits, ids, dweights.contiguous(), **ctx.options), None, None
+        grad = route_experts_backward(logits, ids, dweights.contiguous(), **ctx.options)
+        return without_gradient("the gradient of f8_route", grad, logits, dweights), None, None
 
 
 def f8_route(logits, top_k, **options):

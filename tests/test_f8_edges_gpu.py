@@ -227,3 +227,67 @@ def test_route_scores_below_the_smallest_number(acc, score, tokens, k):  # noqa:
             return (1.5 * e / e.sum(dim=1, keepdim=True) * g64).sum()
         slope = float(value(z + step * direction) - value(z - step * direction)) / (2 * step)
         assert abs(float((grad.double().cpu() * direction).sum()) - slope) <= 1e-5 * float((size * direction.abs()).sum())
+
+
+# ---- gradients that there are none of ----------------------------------------------------------------------------------
+
+def test_a_second_gradient_is_refused(acc):  # noqa: F811
+    """The layer's and the router's gradients have no gradient of their own: asked for one they say so, where a part of it would be missing."""
+    import torch
+    from accera_amd.feed_forward import f8_linear, f8_route
+    x, w = _rand(1, 40, 256).cuda().requires_grad_(), _rand(2, 128, 256).cuda().requires_grad_()
+    for loss in (lambda y: y.square().sum(), lambda y: y.sum()):  # (of the second dx depends on w alone)
+        for at in (0, 1):
+            y = f8_linear(x, w)
+            g = torch.autograd.grad(loss(y), (x, w), create_graph=True)[at]
+            for v in (x, w):
+                with pytest.raises(RuntimeError, match="the gradient of f8_linear has no gradient"):
+                    torch.autograd.grad(y.sum() + g.square().sum(), v, retain_graph=True)
+            with pytest.raises(RuntimeError, match="the gradient of f8_linear has no gradient"):
+                (loss(f8_linear(x, w)) + g.square().sum()).backward()
+        plain = torch.autograd.grad(loss(f8_linear(x, w)), (x, w))
+        again = torch.autograd.grad(loss(f8_linear(x, w)), (x, w), create_graph=True)
+        assert all(torch.equal(a, b) and not a.requires_grad for a, b in zip(plain, again))
+    logits = _rand(3, 40, 16).cuda().requires_grad_()
+    for loss in (lambda v: v.square().sum(), lambda v: v[:, 0].sum()):
+        dlogits, = torch.autograd.grad(loss(f8_route(logits, 4)[1]), logits, create_graph=True)
+        with pytest.raises(RuntimeError, match="the gradient of f8_route has no gradient"):
+            torch.autograd.grad(f8_route(logits, 4)[1].sum() + dlogits.square().sum(), logits)
+
+
+def test_a_gradient_through_the_serving_calls_is_refused(acc):  # noqa: F811
+    """A routed layer, its weighted sum and plain routing have no gradient: where an input asks for one the result is the same, and its gradient is an error, not silently none."""
+    import torch
+    from accera_amd.feed_forward import ExpertLayer
+    tokens, experts, k, hidden, inner = 9, 8, 2, 256, 128
+    dtype = torch.bfloat16
+    x, router = _rand(1, tokens, hidden).to(dtype).cuda(), (_rand(2, hidden, experts) / 16).to(dtype).cuda()
+    layer = ExpertLayer(router, *((_rand(s, experts, inner, hidden) / 16).to(dtype).cuda().requires_grad_() for s in (3, 4)), (_rand(5, experts, hidden, inner) / 12).to(dtype).cuda(), k)
+    want = layer(x)
+    ids, weights = layer.choose(x)
+    plan = acc.plan_experts(ids, experts)
+    rows = _rand(6, tokens * k, hidden).cuda()
+    logits = _rand(7, tokens, experts).cuda()
+    assert not want.requires_grad and not weights.requires_grad
+
+    def ffn(a, b):
+        return acc.expert_ffn_f8(a, ids, b, layer.w13, layer.w13_scale, layer.w2, layer.w2_scale)
+    calls = [("expert_ffn_f8", lambda v: ffn(v, weights), x), ("expert_ffn_f8", lambda v: ffn(x, v), weights), ("combine_experts", lambda v: acc.combine_experts(v, plan, weights), rows),
+             ("combine_experts", lambda v: acc.combine_experts(rows, plan, v), weights), ("route_experts", lambda v: acc.route_experts(v, k)[1], logits),
+             ("ExpertLayer", lambda v: layer(v), x), ("ExpertLayer", lambda v: layer.choose(v)[1], x)]
+    for name, call, value in calls:
+        plain = call(value)
+        leaf = value.detach().clone().requires_grad_()
+        asked = call(leaf)
+        assert torch.equal(asked, plain) and asked.requires_grad and not plain.requires_grad
+        with pytest.raises(RuntimeError, match=f"{name} has no gradient"):
+            (asked.float().sum() + leaf.float().sum()).backward()
+        with torch.no_grad():
+            assert not call(leaf).requires_grad
+    layer.router = router.clone().requires_grad_()
+    with pytest.raises(RuntimeError, match="ExpertLayer has no gradient"):
+        layer(x).float().sum().backward()
+    out = torch.empty_like(x)
+    y = ffn(x.clone().requires_grad_(), weights)
+    given = acc.expert_ffn_f8(x.clone().requires_grad_(), ids, weights, layer.w13, layer.w13_scale, layer.w2, layer.w2_scale, out=out)
+    assert torch.equal(given, y) and given.data_ptr() == out.data_ptr() and given.requires_grad
