@@ -253,6 +253,7 @@ PyObject* route(PyObject* const* a)
         contiguous(bias, "bias");
     }
     const Place place(a[9], logits, {&bias});
+    if (c.top_k > c.experts) check(acc950_route(&c)); // (refused, before memory is taken for it)
     const Tensor ids = place.result({c.tokens, c.top_k}, at::kInt), weights = place.result({c.tokens, c.top_k}, at::kFloat);
     c.logits = data(logits); c.l_row_stride = logits.stride(0);
     c.bias = data(bias); c.ids = data(ids); c.weights = data(weights);
@@ -303,11 +304,12 @@ PyObject* plan(PyObject* const* a)
     c.tokens = ids.size(0); c.top_k = ids.size(1);
     c.experts = integer(a[1]);
     const Place place(a[2], ids, {});
-    const int64_t pairs = c.tokens * c.top_k, need = acc950_expert_plan_workspace(c.tokens, c.top_k, c.experts); // (negative: the call refuses and says why)
-    const Tensor all = place.result({2 * pairs + std::max<int64_t>(c.experts, 0) + 1 + std::max<int64_t>(need, 0) / 4}, at::kInt);
+    const int64_t pairs = c.tokens * c.top_k, need = acc950_expert_plan_workspace(c.tokens, c.top_k, c.experts);
+    if (need < 0) check(acc950_expert_plan(&c)); // (refused, before memory is taken for it)
+    const Tensor all = place.result({2 * pairs + c.experts + 1 + need / 4}, at::kInt);
     int* at = (int*)data(all);
     c.ids = data(ids); c.order = at; c.position = at + pairs; c.offsets = at + 2 * pairs;
-    c.workspace = at + 2 * pairs + std::max<int64_t>(c.experts, 0) + 1;
+    c.workspace = at + 2 * pairs + c.experts + 1;
     c.stream = place.stream;
     check(acc950_expert_plan(&c));
     return wrap(all);

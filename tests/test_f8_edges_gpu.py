@@ -291,3 +291,15 @@ def test_a_gradient_through_the_serving_calls_is_refused(acc):  # noqa: F811
     y = ffn(x.clone().requires_grad_(), weights)
     given = acc.expert_ffn_f8(x.clone().requires_grad_(), ids, weights, layer.w13, layer.w13_scale, layer.w2, layer.w2_scale, out=out)
     assert torch.equal(given, y) and given.data_ptr() == out.data_ptr() and given.requires_grad
+
+
+def test_refusals_come_before_any_memory(acc):  # noqa: F811
+    """Sizes that no call takes are refused as such, however much memory their results would be."""
+    import torch
+    ids = torch.zeros((4, 2), dtype=torch.int32, device="cuda")
+    before = torch.cuda.max_memory_allocated()
+    with pytest.raises(acc.Acc950Error, match="experts"):
+        acc.plan_experts(ids, 1 << 33)
+    with pytest.raises(acc.Acc950Error, match="top_k"):
+        acc.route_experts(torch.zeros((4, 8), device="cuda"), 1 << 33)
+    assert torch.cuda.max_memory_allocated() < before + (1 << 30)
