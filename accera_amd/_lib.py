@@ -29,8 +29,8 @@ EXPORTS = [
     "acc950_bound_choice", "acc950_host_parts", "acc950_workspace_probe", "acc950_allocation_probe", "acc950_release_workspaces",
 ]
 # feed-forward operators in 8-bit floating point (include/accera_mi355x_f8.h), in the same library
-F8_EXPORTS = ["acc950_f8_quantize", "acc950_f8_gemm", "acc950_f8_gemm_workspace", "acc950_route", "acc950_route_backward", "acc950_expert_plan", "acc950_expert_plan_workspace",
-              "acc950_f8_expert_gemm", "acc950_expert_combine", "acc950_f8_expert_ffn", "acc950_f8_expert_ffn_workspace"]
+F8_EXPORTS = ["acc950_f8_quantize", "acc950_f8_gemm", "acc950_f8_gemm_workspace", "acc950_route", "acc950_route_backward", "acc950_expert_plan", "acc950_expert_plan_within", "acc950_expert_plan_workspace",
+              "acc950_f8_expert_gemm", "acc950_expert_combine", "acc950_f8_expert_ffn", "acc950_f8_expert_ffn_within", "acc950_f8_expert_ffn_workspace"]
 # measurement aids (include/accera_mi355x_probes.h, libaccera_mi355x_probes.so): not part of the product
 PROBE_EXPORTS = ["acc950_mfma_ceiling", "acc950_mfma_traffic_probe", "acc950_mfma_phase_probe", "acc950_copy_probe", "acc950_stream_read_probe",
                  "acc950_probes_last_error"]
@@ -84,9 +84,9 @@ def lib():
     for name in EXPORTS:
         if name != "acc950_last_error":
             getattr(L, name).restype = ci
-    for name in F8_EXPORTS:  # arguments in a packed struct, or sizes alone
+    for name in F8_EXPORTS:  # arguments in a packed struct (and the bytes of a workspace), or sizes alone
         size = {"acc950_expert_plan_workspace": 3, "acc950_f8_expert_ffn_workspace": 5}.get(name)
-        getattr(L, name).argtypes = [i64] * size if size else [vp]
+        getattr(L, name).argtypes = [i64] * size if size else [vp, i64] if name.endswith("_within") else [vp]
         getattr(L, name).restype = i64 if name.endswith("_workspace") else ci
     _lib = L
     return L

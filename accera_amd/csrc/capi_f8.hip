@@ -308,11 +308,14 @@ extern "C" int64_t acc950_expert_plan_workspace(int64_t tokens, int64_t top_k, i
     return expert_plan_workspace(tokens * top_k, experts);
 }
 
-extern "C" int acc950_expert_plan(const acc950_expert_plan_call* c)
+extern "C" int acc950_expert_plan(const acc950_expert_plan_call* c) { return acc950_expert_plan_within(c, INT64_MAX); }
+
+extern "C" int acc950_expert_plan_within(const acc950_expert_plan_call* c, int64_t workspace_bytes)
 {
     if (!c) return refuse("null call");
     const int64_t need = acc950_expert_plan_workspace(c->tokens, c->top_k, c->experts);
     if (need < 0) return refuse("a plan takes 1 to 1024 experts, top_k of 1 to 64, and a number of pairs below 2^31 - 1024");
+    if (workspace_bytes < need) return refuse("the workspace is smaller than the plan's");
     if (!c->offsets || (c->tokens > 0 && (!c->ids || !c->order || !c->position)) || (need > 0 && !c->workspace)) return refuse("null pointer");
     if (misaligned(c->ids, 4) || misaligned(c->order, 4) || misaligned(c->position, 4) || misaligned(c->offsets, 4) || misaligned(c->workspace, 4))
         return refuse("a pointer is not aligned to its element type");
@@ -424,7 +427,9 @@ extern "C" int64_t acc950_f8_expert_ffn_workspace(int64_t tokens, int64_t hidden
     return ffn_layout(tokens, hidden, inner, experts, top_k).bytes;
 }
 
-extern "C" int acc950_f8_expert_ffn(const acc950_f8_expert_ffn_call* c)
+extern "C" int acc950_f8_expert_ffn(const acc950_f8_expert_ffn_call* c) { return acc950_f8_expert_ffn_within(c, INT64_MAX); }
+
+extern "C" int acc950_f8_expert_ffn_within(const acc950_f8_expert_ffn_call* c, int64_t workspace_bytes)
 {
     if (!c) return refuse("null call");
     if (c->type != ACC950_F16 && c->type != ACC950_BF16) return refuse("a routed layer takes fp16 and bf16");
@@ -440,6 +445,7 @@ extern "C" int acc950_f8_expert_ffn(const acc950_f8_expert_ffn_call* c)
     if (misaligned(c->w13, 16) || misaligned(c->w2, 16)) return refuse("the experts' matrices must start on 16-byte boundaries");
     const int64_t pairs = c->tokens * c->top_k, hb = blocks_of(c->hidden), ib = blocks_of(c->inner);
     const FfnLayout l = ffn_layout(c->tokens, c->hidden, c->inner, c->experts, c->top_k);
+    if (workspace_bytes < l.bytes) return refuse("the workspace is smaller than the layer's");
     char* ws = (char*)c->workspace;
     const hipStream_t stream = (hipStream_t)c->stream;
 

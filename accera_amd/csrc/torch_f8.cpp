@@ -311,7 +311,7 @@ PyObject* plan(PyObject* const* a)
     c.ids = data(ids); c.order = at; c.position = at + pairs; c.offsets = at + 2 * pairs;
     c.workspace = at + 2 * pairs + c.experts + 1;
     c.stream = place.stream;
-    check(acc950_expert_plan(&c));
+    check(acc950_expert_plan_within(&c, need));
     return wrap(all);
 }
 
@@ -413,7 +413,7 @@ PyObject* expert_ffn(PyObject* const* a)
     c.y = data(out); c.y_row_stride = out.stride(0);
     c.workspace = data(workspace);
     c.stream = place.stream;
-    check(acc950_f8_expert_ffn(&c));
+    check(acc950_f8_expert_ffn_within(&c, workspace.numel()));
     return wrap(out);
 }
 

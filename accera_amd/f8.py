@@ -180,7 +180,7 @@ def expert_ffn_f8(x, ids, weights, w13, w13_scale, w2, w2_scale, out=None, works
     x (tokens, hidden) fp16 / bf16; ids, weights as route_experts gives them (an id outside 0 .. experts - 1: no expert).  w13 (experts, 2, inner, hidden):
     gate and up, w2 (experts, hidden, inner), e4m3 with scales of 128 x 128 blocks, contiguous.  q quantises rows with power-of-two scales, so that the inner values
     are rounded once, to their codes; all sums are fp32.  ``workspace``: a uint8 tensor of
-    at least expert_ffn_workspace(...) bytes to be used over and over, or None to allocate one.
+    at least expert_ffn_workspace(...) bytes to be used over and over (on one stream: calls that may run at the same time take one each), or None to allocate one.
     """
     y = _native.expert_ffn(x, ids, weights, w13, w13_scale, w2, w2_scale, out, workspace, _raw(stream))
     return without_gradient("expert_ffn_f8", y, x, weights) if x.requires_grad or weights.requires_grad else y

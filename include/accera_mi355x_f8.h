@@ -10,7 +10,8 @@
  * asynchronous launch on `stream` (a hipStream_t, or NULL for the default stream), an ACC950_* status and
  * acc950_last_error() for its text.  No call allocates device memory or waits for the device, so all may be captured into a graph
  * (after one call outside it: the first launch of a kernel loads its code).  Scratch memory is the caller's; a call that takes
- * some says how much in the function beside it.  Arguments come in a struct, read before the function returns.
+ * some says how much in the function beside it, and calls that may run at the same time (on two streams) take a piece each.  Arguments come in a
+ * struct, read before the function returns.
  * None of these has a counterpart in the reference, whose tensorized plans end at 16-bit and int8 inputs
  * (accera/python/accera/Targets.py:796-821).
  */
@@ -134,7 +135,8 @@ int acc950_route_backward(const acc950_route_backward_call* call);
 /*
  * Order of the tokens * top_k (token, slot) pairs by expert, those of one expert in their own order, pairs without an expert
  * (-1, or any number outside 0 .. experts - 1) last: order[r] = pair of sorted row r, position[pair] = its row (-1: none), offsets[e] = first row of
- * expert e (experts + 1 of them; the last is the number of rows).  All int32.  `workspace` holds acc950_expert_plan_workspace bytes.
+ * expert e (experts + 1 of them; the last is the number of rows).  All int32.  `workspace` holds acc950_expert_plan_workspace bytes,
+ * which acc950_expert_plan takes on trust and acc950_expert_plan_within checks.
  */
 typedef struct acc950_expert_plan_call {
     const void* ids;
@@ -146,6 +148,7 @@ typedef struct acc950_expert_plan_call {
     void* stream;
 } acc950_expert_plan_call;
 int acc950_expert_plan(const acc950_expert_plan_call* call);
+int acc950_expert_plan_within(const acc950_expert_plan_call* call, int64_t workspace_bytes);
 int64_t acc950_expert_plan_workspace(int64_t tokens, int64_t top_k, int64_t experts);
 
 /*
@@ -193,7 +196,9 @@ int acc950_expert_combine(const acc950_expert_combine_call* call);
  * with power-of-two scales and e = ids[t, slot].  x and y: tokens x hidden of `type` F16 / BF16.  w13: (experts, 2, inner, hidden) e4m3 -- gate
  * and up --, scales (experts, 2, ceil(inner / 128), ceil(hidden / 128)); w2: (experts, hidden, inner), scales
  * (experts, ceil(hidden / 128), ceil(inner / 128)); all contiguous, w13 and w2 from 16-byte boundaries on.  Sums are fp32, rounded once, to `type`.
- * `workspace` holds acc950_f8_expert_ffn_workspace bytes, 256-byte aligned.
+ * `workspace` holds acc950_f8_expert_ffn_workspace bytes, 256-byte aligned;
+ * acc950_f8_expert_ffn takes that on trust, acc950_f8_expert_ffn_within checks it.  It needs no clearing and may be used again by calls that follow each other on
+ * a stream, but not by two that may run at the same time: steps' results and the counters that hand out tiles lie there.
  */
 typedef struct acc950_f8_expert_ffn_call {
     int64_t type, tokens, hidden, inner, experts, top_k;
@@ -211,6 +216,7 @@ typedef struct acc950_f8_expert_ffn_call {
     void* stream;
 } acc950_f8_expert_ffn_call;
 int acc950_f8_expert_ffn(const acc950_f8_expert_ffn_call* call);
+int acc950_f8_expert_ffn_within(const acc950_f8_expert_ffn_call* call, int64_t workspace_bytes);
 int64_t acc950_f8_expert_ffn_workspace(int64_t tokens, int64_t hidden, int64_t inner, int64_t experts, int64_t top_k);
 
 #if defined(__cplusplus)

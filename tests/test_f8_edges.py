@@ -1,0 +1,28 @@
+"""C ABI, build and documents of the feed-forward operators in 8-bit floating point, on the host alone: no call here gets as far as a launch."""
+import struct
+
+import pytest
+
+from accera_amd import _lib
+from test_f8_abi import GOOD, _fields
+
+
+def _packed(entry, **change):
+    args = dict(GOOD[entry], **change)
+    fields = _fields(entry + "_call")
+    return struct.pack("".join("d" if d else "Q" if p else "q" for _, d, p in fields), *(args[n] for n, _, _ in fields))
+
+
+@pytest.mark.parametrize("entry,sizes", [("acc950_expert_plan", ("tokens", "top_k", "experts")), ("acc950_f8_expert_ffn", ("tokens", "hidden", "inner", "experts", "top_k"))])
+def test_a_workspace_that_is_too_small_is_refused(entry, sizes):
+    L = _lib.lib()
+    need = getattr(L, entry + "_workspace")(*(GOOD[entry][n] for n in sizes))
+    assert need > 0
+    for smaller in (need - 1, 1, 0, -1):
+        assert getattr(L, entry + "_within")(_packed(entry), smaller) == _lib.INVALID_ARGUMENT
+        assert b"workspace is smaller" in L.acc950_last_error()
+    assert getattr(L, entry + "_within")(None, need) == _lib.INVALID_ARGUMENT
+    # a size that the call does not take, whatever the workspace; nothing to do
+    assert getattr(L, entry + "_within")(_packed(entry, experts=2000), 1 << 60) == _lib.INVALID_ARGUMENT and b"1024 experts" in L.acc950_last_error()
+    if entry == "acc950_f8_expert_ffn":
+        assert L.acc950_f8_expert_ffn_within(_packed(entry, tokens=0), 0) == _lib.OK
