@@ -25,15 +25,18 @@ bool misaligned(const void* p, size_t to) { return (reinterpret_cast<uintptr_t>(
 size_t type_bytes(int64_t t) { return t == ACC950_F32 ? 4 : 2; }
 int64_t blocks_of(int64_t n) { return (n + F8_BLOCK - 1) / F8_BLOCK; }
 
+// Whether bytes lie within 32-bit offsets from the first of `rows` rows: these and `more` of the last one (which may be more than the rows are apart).
+bool offsets_in_32_bits(int64_t rows, int64_t stride, int64_t more) { return more < 1ll << 32 && stride <= ((1ll << 32) - 1 - more) / rows; }
+
 // Whether the kernels that fetch 16 bytes at a time take the problem: A and B contiguous along K with rows on 16-byte boundaries (the
 // rows' own padding is read where K ends inside 16 bytes, never used), C's columns contiguous, and 32-bit offsets from the row a tile
-// starts at -- from A's first row where a plan picks the rows (one for every top_k pairs).
+// starts at (it has 256 at most) -- from A's first row where a plan picks the rows (one for every top_k pairs).
 bool vectors_can_take(const F8GemmArgs& g)
 {
     if (g.K == 0 || g.a_cs != 1 || g.b_rs != 1 || (g.c_cs != 1 && g.N > 1)) return false;
     if ((g.a_rs | g.b_cs | g.b_es) % 16 || misaligned(g.A, 16) || misaligned(g.B, 16)) return false;
-    const int64_t a_rows = g.offsets && g.gather ? (g.M + g.top_k - 1) / g.top_k : 256, most = 1ll << 32;
-    return a_rows * g.a_rs < most && a_rows * g.as_rs * 4 < most && 256 * g.b_cs < most && 256 * g.bs_cs * 4 < most;
+    const int64_t a_rows = g.offsets && g.gather ? (g.M + g.top_k - 1) / g.top_k : g.M < 256 ? g.M : 256, b_cols = g.N < 256 ? g.N : 256;
+    return offsets_in_32_bits(a_rows, g.a_rs, g.K) && offsets_in_32_bits(a_rows * 4, g.as_rs, 4) && offsets_in_32_bits(b_cols, g.b_cs, g.K) && offsets_in_32_bits(b_cols * 4, g.bs_cs, 4);
 }
 
 // Operands that those kernels do not take as they lie can be laid out anew in scratch memory, where nothing but their strides and alignment is in the way.
@@ -374,11 +377,11 @@ extern "C" int acc950_expert_combine(const acc950_expert_combine_call* c)
 namespace {
 
 // Whether the gate and up product of a routed layer goes through the kernels that end in codes: whole 16-byte pieces of K, 32-bit offsets
-// from x's first row, and from the gate's scales to the up matrix's.
+// from x's first row, from a tile's first column in the weights, and from the gate's scales to the up matrix's.
 bool ends_in_codes(int64_t tokens, int64_t hidden, int64_t inner)
 {
     const int64_t most = 1ll << 32;
-    return hidden % 16 == 0 && tokens * hidden < most && tokens * 4 < most && blocks_of(inner + 256) * blocks_of(hidden) * 4 < most;
+    return hidden % 16 == 0 && tokens * hidden < most && tokens * 4 < most && 256 * hidden < most && blocks_of(inner + 256) * blocks_of(hidden) * 4 < most;
 }
 
 // Where the steps of a routed layer keep their results in its workspace (bytes from its start).

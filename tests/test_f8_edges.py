@@ -38,3 +38,26 @@ def test_the_c_library_is_built_without_torch(python, binding):
     assert out.returncode == 0, out.stderr[-500:]
     assert "-o ../lib/libaccera_mi355x.so" in out.stdout and "-o ../lib/libaccera_mi355x_probes.so" in out.stdout
     assert ("-o ../lib/_torch_f8.so" in out.stdout) == binding and ("is left out" in out.stdout) != binding
+
+
+def test_offsets_past_32_bits_go_to_the_kernels_that_hold_them():
+    """What the kernels with 32-bit offsets from a tile's first row cannot reach, told by the scratch memory that the other path takes."""
+    def layer(hidden):
+        return _lib.lib().acc950_f8_expert_ffn_workspace(1, hidden, 128, 1, 1)
+
+    def codes_only(hidden):  # every step's results but the gate and up product's in fp32
+        up = lambda n: -(-n // 256) * 256  # noqa: E731
+        return 6 * 256 + up(hidden) + up(hidden // 128 * 4) + up(4 * hidden) + up(hidden // 64 * 2 * 4)
+    small, large = (1 << 24) - 128, 1 << 25
+    assert layer(small) == codes_only(small) and layer(large) == codes_only(large) + 2 * 128 * 4
+
+    def product(**change):
+        return getattr(_lib.lib(), "acc950_f8_gemm_workspace")(_packed("acc950_f8_gemm", **{**dict(out_type=_lib.F32, M=256, N=512, K=1 << 20, a_row_stride=1 << 20, b_col_stride=1 << 20,
+                                                                                                  as_block_stride=256, bs_col_stride=1 << 13, c_row_stride=512), **change}))
+    assert product() > 0  # (slices of K)
+    # rows that overlap (a matrix of all windows of a long row): the last one ends far behind its start
+    far = (1 << 24) - 16
+    assert product(a_row_stride=16) > 0 and product(K=1 << 25, b_col_stride=far, a_row_stride=16, bs_col_stride=1 << 18) == 0
+    assert product(K=1 << 25, b_col_stride=16, a_row_stride=far, bs_col_stride=1 << 18) == 0
+    # strides whose product with a tile's rows passes 64 bits
+    assert product(a_row_stride=1 << 56) == 0 and product(b_col_stride=1 << 56) == 0 and product(as_row_stride=1 << 54) == 0

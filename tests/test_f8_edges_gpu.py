@@ -2,7 +2,7 @@
 import numpy as np
 import pytest
 
-from test_f8_gpu import U, _apart, _codes, _dtype, _rand, _route64, _scales, _spread, acc  # noqa: F401
+from test_f8_gpu import U, _apart, _check_product, _codes, _dtype, _product64, _rand, _route64, _scales, _spread, acc  # noqa: F401
 
 pytestmark = pytest.mark.gpu
 
@@ -303,3 +303,30 @@ def test_refusals_come_before_any_memory(acc):  # noqa: F811
     with pytest.raises(acc.Acc950Error, match="top_k"):
         acc.route_experts(torch.zeros((4, 8), device="cuda"), 1 << 33)
     assert torch.cuda.max_memory_allocated() < before + (1 << 30)
+
+
+# ---- products ----------------------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("m", [1, 3, 20])
+def test_rows_far_apart_and_rows_that_overlap(acc, m):  # noqa: F811
+    """The last tokens of some long sequences (rows 16 MiB and more apart), one row's windows (rows that lie over one another), a weight of few columns far apart."""
+    import torch
+    k, n = 272, 130
+    a, w, sa, sw = _codes(1, m, k), _codes(2, n, k), _scales(3, m, 3), _scales(4, 2, 3)
+    want = _product64(a, sa, w, sw, 128)
+    far = torch.zeros((m, (1 << 24) + 16), dtype=torch.float8_e4m3fn, device="cuda")
+    far[:, -k:] = a.cuda()
+    for rows in (far[:, -k:], far[:, -k:].as_strided((m, k), (far.stride(0) if m > 1 else 1 << 56, 1))):
+        for kind in ("f32", "bf16"):
+            c = torch.full((m, n), 7.0, dtype=_dtype(kind), device="cuda")
+            acc.gemm_f8(rows, sa.cuda(), w.cuda().t(), sw.cuda().t(), c)
+            _check_product(c, *want, k, kind)
+            c = torch.full((n, m), 7.0, dtype=_dtype(kind), device="cuda")  # (the same rows as the columns of B, a factor for each)
+            acc.gemm_f8(w.cuda(), _scales(5, n, 3).cuda(), rows.t(), sa.cuda().t(), c)
+            _check_product(c, *_product64(w, _scales(5, n, 3), a, sa, 1), k, kind)
+    long = _codes(6, 1, 16 * m + k)
+    windows = torch.stack([long[0, 16 * i:16 * i + k].view(torch.uint8) for i in range(m)]).view(long.dtype)
+    for kind in ("f32", "bf16"):
+        c = torch.full((m, n), 7.0, dtype=_dtype(kind), device="cuda")
+        acc.gemm_f8(long.cuda().as_strided((m, k), (16, 1)), sa.cuda(), w.cuda().t(), sw.cuda().t(), c)
+        _check_product(c, *_product64(windows, sa, w, sw, 128), k, kind)
