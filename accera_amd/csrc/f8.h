@@ -48,7 +48,7 @@ struct F8GemmArgs {
     int* tickets;         // 8 counters, zero at the launch (f8_tile_by_ticket), or null
     // gated: B's second matrix (up) lies b_up elements behind the first (gate), its scales bs_up; C takes codes, out_scale their scales.
     // Not gated, tiles of experts' rows, out_type fp16: with out_scale C takes fp16 values, whose row has a power of two for each 32 columns at
-    // out_scale + row * os_rs (even).
+    // out_scale + row * os_rs (even); such rows have no weights.
     int64_t b_up, bs_up;
     float* out_scale;
     int64_t os_rs, os_bs;

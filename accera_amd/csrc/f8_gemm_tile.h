@@ -256,7 +256,6 @@ __device__ __forceinline__ void f8_write_tile(const F8GemmArgs& p, f32x4 (&acc)[
                 float top = 0.f; // (NaN aside: it stays what it is)
 #pragma unroll
                 for (int j = 0; j < TN; ++j) {
-                    if (p.row_weights) acc[i][j] *= w;
                     if (!whole) {
 #pragma unroll
                         for (int e = 0; e < 4; ++e)
