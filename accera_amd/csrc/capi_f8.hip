@@ -464,8 +464,10 @@ extern "C" int acc950_f8_expert_ffn_within(const acc950_f8_expert_ffn_call* c, i
     if (int rc = ended(launch_expert_plan_and_quantize(plan, q, stream), "the plan of the experts' rows")) return rc;
 
     // The inner values are not rounded before they become codes: half a unit of fp16 already moves 1 in 500 of them across a boundary between
-    // two codes.  The e4m3 instruction's sums (2^-16) move 1 in 5000, which a bf16 result does not show; a fp16 result's gate and up
-    // products take the fp32 sums.
+    // two codes.  The e4m3 instruction's sums (2^-16) move 1 in 5000, and 1 in 30000 of a row's scales.  With few rows to an expert, where the weights' bytes are what takes the
+    // time, both products have fp32 sums (us with / without, 64 experts of 2048x1024: 8 tokens 47.0 / 47.0, 120 115.4 / 114.6; 20 of 1040x720: 8 tokens 23.2 / 21.8).  With
+    // more, the gate and up product of a fp16 layer has, and that of a bf16 layer has not: it would cost 100 of 304 us (4096 tokens), 16 of 156 (1024), for an
+    // error against the same layer in 64 bits of 1.7e-3, which is bf16's own rounding, and not 2.0e-3.
     const bool wide = c->type == ACC950_F16;
     F8GemmArgs g{};
     g.A = q.q; g.a_rs = q.q_rs; g.a_cs = 1; g.a_scale = q.scale; g.as_rs = q.s_rs; g.as_ks = q.s_bs;
@@ -477,7 +479,7 @@ extern "C" int acc950_f8_expert_ffn_within(const acc950_f8_expert_ffn_call* c, i
     g.out_scale = (float*)(ws + l.h_scale); g.os_rs = 1; g.os_bs = pairs;
     g.tickets = plan.zeros;
     if (c->inner > 0 && ends_in_codes(c->tokens, c->hidden, c->inner)) {
-        if (int rc = ended(rows_of_matrix(g) <= FEW_ROWS ? launch_f8_gated_few(g, wide, stream) : launch_f8_gated_tile(g, wide, stream), "gate and up product")) return rc;
+        if (int rc = ended(rows_of_matrix(g) <= FEW_ROWS ? launch_f8_gated_few(g, stream) : launch_f8_gated_tile(g, wide, stream), "gate and up product")) return rc;
     } else if (c->inner > 0) {
         // gate | up in fp32, then the activation
         F8GemmArgs half = g;
@@ -503,7 +505,8 @@ extern "C" int acc950_f8_expert_ffn_within(const acc950_f8_expert_ffn_call* c, i
     g.out_type = halves ? T_F16 : T_F32;
     g.out_scale = halves ? (float*)(ws + l.row_scale) : nullptr; g.os_rs = (c->hidden + 63) / 64 * 2;
     g.gather = 0; g.tickets = plan.zeros + 8;
-    if (int rc = run_gemm(g, ACC950_VARIANT_AUTO, false, 1, nullptr, 0, stream)) return rc;
+    const bool few = rows_of_matrix(g) <= FEW_ROWS; // (else the e4m3 instruction: 2^-16 of a row beside 2^-12 or 2^-9 of the result)
+    if (int rc = run_gemm(g, ACC950_VARIANT_AUTO, few, 1, nullptr, 0, stream)) return rc;
 
     CombineArgs y{};
     y.x = ws + l.rows; y.x_rs = c->hidden; y.position = plan.position; y.y = c->y; y.y_rs = c->y_row_stride;

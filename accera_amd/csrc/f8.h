@@ -123,7 +123,7 @@ hipError_t launch_f8_gemm_tile(const F8GemmArgs& a, int tile, bool wide, hipStre
 hipError_t launch_f8_add_slices(const F8GemmArgs& a, hipStream_t s);
 constexpr int F8_FEW_FORMS = 2;
 hipError_t launch_f8_gemm_few(const F8GemmArgs& a, int form, bool wide, hipStream_t s);
-hipError_t launch_f8_gated_few(const F8GemmArgs& a, bool wide, hipStream_t s);
+hipError_t launch_f8_gated_few(const F8GemmArgs& a, hipStream_t s);
 hipError_t launch_f8_gated_tile(const F8GemmArgs& a, bool wide, hipStream_t s);
 hipError_t launch_route(const RouteArgs& a, hipStream_t s);
 hipError_t launch_route_backward(const RouteArgs& a, hipStream_t s);
@@ -234,7 +234,7 @@ __device__ __forceinline__ float silu_mul(float gate, float up)
     return gate * __builtin_amdgcn_rcpf(1.f + (fabsf(t) < 128.f ? fmaf(e, rest * 0.693147182f, e) : e)) * up;
 }
 
-// The same for values that become codes at once, half the instructions: the exponent's own rounding moves exp(-gate) by |gate| * 2^-24 of itself, no more than
+// The same for values that become codes at once behind sums of the e4m3 instruction, half the instructions: the exponent's own rounding moves exp(-gate) by |gate| * 2^-24 of itself, no more than
 // what the sums of the e4m3 instruction bring along, and 1 in 10^5 of the codes across a boundary.
 __device__ __forceinline__ float silu_mul_to_code(float gate, float up)
 {

@@ -218,7 +218,7 @@ __global__ void __launch_bounds__(Cfg::NT) f8_gemm_few_kernel(F8GemmArgs p)
                 unsigned top = 0;
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    h[i][e] = c + e < p.N ? silu_mul_to_code(acc[i][0][e], acc[i][1][e]) : 0.f;
+                    h[i][e] = c + e < p.N ? silu_mul(acc[i][0][e], acc[i][1][e]) : 0.f;
                     top = max(top, __float_as_uint(h[i][e]) & 0x7fffffffu);
                 }
                 top = f8_max_over(top, 16);

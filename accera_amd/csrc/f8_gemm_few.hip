@@ -22,10 +22,6 @@ hipError_t launch_f8_gemm_few(const F8GemmArgs& a, int form, bool wide, hipStrea
     return form == 0 ? run<1, 1, 1, 4, 4>(a, wide, s) : run<1, 2, 4, 1, 4>(a, wide, s);
 }
 
-hipError_t launch_f8_gated_few(const F8GemmArgs& a, bool wide, hipStream_t s)
-{
-    return wide ? launch_f8_few<F8FewConfig<1, 2, 8, 1, 4, true, false, true, true>>(a, s)
-                : launch_f8_few<F8FewConfig<1, 2, 8, 1, 4, false, false, true, true>>(a, s);
-}
+hipError_t launch_f8_gated_few(const F8GemmArgs& a, hipStream_t s) { return launch_f8_few<F8FewConfig<1, 2, 8, 1, 4, true, false, true, true>>(a, s); }
 
 } // namespace acc950

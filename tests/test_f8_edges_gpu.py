@@ -2,7 +2,7 @@
 import numpy as np
 import pytest
 
-from test_f8_gpu import U, _apart, _check_product, _codes, _dtype, _product64, _rand, _route64, _scales, _spread, acc  # noqa: F401
+from test_f8_gpu import U, _apart, _check_product, _codes, _dtype, _expert_ids, _product64, _rand, _route64, _scales, _spread, acc  # noqa: F401
 
 pytestmark = pytest.mark.gpu
 
@@ -330,3 +330,33 @@ def test_rows_far_apart_and_rows_that_overlap(acc, m):  # noqa: F811
         c = torch.full((m, n), 7.0, dtype=_dtype(kind), device="cuda")
         acc.gemm_f8(long.cuda().as_strided((m, k), (16, 1)), sa.cuda(), w.cuda().t(), sw.cuda().t(), c)
         _check_product(c, *_product64(windows, sa, w, sw, 128), k, kind)
+
+
+# ---- a routed layer ----------------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("tokens,k,experts,hidden,inner", [(8, 6, 64, 512, 256), (20, 3, 6, 272, 400), (1, 2, 8, 256, 128), (90, 4, 24, 384, 272), (16, 2, 4, 1040, 720)])
+@pytest.mark.parametrize("kind", ["f16", "bf16"])
+def test_a_layer_with_few_rows_has_sums_in_fp32(acc, tokens, k, experts, hidden, inner, kind):  # noqa: F811
+    """Up to 16 rows for each expert the layer is that of fp32 products by single calls.  Their sums' order moves 2 * 2^-20 / 2^-4 of the inner values (2^-20: a sum's error, 2^-4: a code's
+    step) to another code, and with one of them all of a token's results by their own rounding: 2^-15 * inner * k of the tokens, 5 % here at most.  (The e4m3 instruction's sums
+    move half or more of them.)"""
+    import torch
+    ids = torch.from_numpy(_expert_ids(hidden, tokens, k, experts)).cuda()
+    x = (_rand(1, tokens, hidden) * torch.exp(_rand(2, tokens, 1))).to(_dtype(kind)).cuda()
+    w13, w2 = _codes(3, experts, 2, inner, hidden).cuda(), _codes(4, experts, hidden, inner).cuda()
+    hb, ib = -(-hidden // 128), -(-inner // 128)
+    s13, s2 = (0.002 * _scales(5, experts, 2, ib, hb)).cuda(), (0.02 * _scales(6, experts, hb, ib)).cuda()
+    weights = torch.rand(tokens, k, generator=torch.Generator().manual_seed(7)).cuda()
+    got = acc.expert_ffn_f8(x, ids, weights, w13, s13, w2, s2)
+    plan = acc.plan_experts(ids, experts)
+    xq, xs = acc.quantize_f8(x, power_of_two=True)
+    h, rows = torch.zeros((tokens * k, 2 * inner), device="cuda"), torch.empty((tokens * k, hidden), device="cuda")
+    for half in (0, 1):
+        acc.expert_gemm_f8(xq, xs, w13[:, half].transpose(1, 2), s13[:, half].transpose(1, 2), plan, h[:, half * inner:(half + 1) * inner], gather=True)
+    hq, hs = acc.quantize_f8(h, activation="silu_mul", power_of_two=True)
+    acc.expert_gemm_f8(hq, hs, w2.transpose(1, 2), s2.transpose(1, 2), plan, rows, gather=False)
+    want = acc.combine_experts(rows, plan, weights)
+    assert torch.isfinite(want).all() and float(want.abs().max()) < 6e4
+    moved = (got != want.to(got.dtype)).float().mean(dim=1)
+    same = (moved < 0.02).float().mean()  # (of a token's results: those whose rounding the sums' last bits change, 2 * 2^-20 / 2^-11 and less)
+    assert same >= 1 - max(0.05, 1.5 / tokens), (float(same), moved.tolist())
