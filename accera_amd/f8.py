@@ -99,13 +99,16 @@ def quantize_f8(x, out=None, scale=None, *, group_rows=1, transpose=False, activ
 
 
 def gemm_f8(A, a_scale, B, b_scale, C, epilogue=_lib.EPILOGUE_NONE, variant=_lib.VARIANT_AUTO, k_slices=0, stream=None):
-    """C = epilogue(A @ B) of e4m3 operands with block scales, in place on C (fp32 / fp16 / bf16), asynchronously; fp32 sums.
+    """C = epilogue(A @ B) of e4m3 operands with block scales, in place on C (fp32 / fp16 / bf16), asynchronously.
 
     A (M, K) with a_scale (M, ceil(K / 128)); B (K, N) with b_scale (ceil(K / 128), ceil(N / 128)), or (ceil(K / 128), N) for scales of single columns
     (as many columns as rows of b_scale are told apart by N; where both are the same, N = 1, they are the same thing).  ``epilogue``: NONE
     or RELU.  B is commonly ``wq.t()`` of a weight quantised by rows, b_scale ``ws.t()``.  Strides are honoured; operands that are
     contiguous along K, with rows on 16-byte boundaries (as quantize_f8 leaves them), are taken as they lie, others laid out anew first.  A small result with a long sum is computed in slices
     of K, added in a fixed order; ``variant`` and ``k_slices`` name a kernel and a number of slices (of a tile kernel) instead.
+
+    A fp32 C has fp32 sums.  fp16 and bf16 ones are computed twice as fast on the e4m3 matrix instruction, whose sums inside a block of 128 drop what lies below 2^-13 of the
+    largest of eight terms: 2^-16 of the result, more where terms cancel.  Where that matters take a fp32 C, or name a variant with fp32 sums (0, 6 to 8, 18, 19).
     """
     _native.gemm(A, a_scale, B, b_scale, C, epilogue, variant, k_slices, _raw(stream))
     return C
@@ -179,7 +182,8 @@ def expert_ffn_f8(x, ids, weights, w13, w13_scale, w2, w2_scale, out=None, works
 
     x (tokens, hidden) fp16 / bf16; ids, weights as route_experts gives them (an id outside 0 .. experts - 1: no expert).  w13 (experts, 2, inner, hidden):
     gate and up, w2 (experts, hidden, inner), e4m3 with scales of 128 x 128 blocks, contiguous.  q quantises rows with power-of-two scales, so that the inner values
-    are rounded once, to their codes; all sums are fp32.  ``workspace``: a uint8 tensor of
+    are rounded once, to their codes.  Up to 16 rows for each expert all sums are fp32; with more, some are the e4m3 instruction's (see gemm_f8: the gate and up product's of a bf16 layer,
+    the down product's), and a bf16 layer's rows are fp16 with shared powers of two until they are added up, in fp32.  ``workspace``: a uint8 tensor of
     at least expert_ffn_workspace(...) bytes to be used over and over (on one stream: calls that may run at the same time take one each), or None to allocate one.
     """
     y = _native.expert_ffn(x, ids, weights, w13, w13_scale, w2, w2_scale, out, workspace, _raw(stream))

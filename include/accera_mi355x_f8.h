@@ -55,7 +55,10 @@ int acc950_f8_quantize(const acc950_f8_quantize_call* call);
 
 /*
  * C[i, j] = epilogue(sum over blocks b of a_scale[i, b] * b_scale[b, j / group_cols] * sum over k in b of A[i, k] * B[k, j]),
- * fp32 sums, out_type F32 / F16 / BF16; epilogue ACC950_EPILOGUE_NONE or _RELU; group_cols 128 or 1.
+ * out_type F32 / F16 / BF16; epilogue ACC950_EPILOGUE_NONE or _RELU; group_cols 128 or 1.
+ * Sums: blocks are added in fp32, always.  Inside a block, F32 results have fp32 sums throughout.  F16 and BF16 ones are left to the e4m3 matrix
+ * instruction, twice as fast, which adds its products eight at a time and drops what lies below 2^-13 of the largest of them (2^16 + 2^2 gives 2^16): 2^-16 of a sum
+ * of random terms, but 2^-13 of its largest terms where they cancel.  For fp32 sums take an F32 result, or one of the variants that name them below.
  * With B = W^T for a weight W quantised in 128 x 128 blocks this is a layer's forward product; with W quantised transposed the
  * gradient of its input; with both operands quantised transposed and group_cols 1 the gradient of W.
  * Any sizes, strides and alignments; fast where A and B are contiguous along K and their rows start on 16-byte boundaries.  Where they are not, they
@@ -84,7 +87,7 @@ typedef struct acc950_f8_gemm_call {
 } acc950_f8_gemm_call;
 int acc950_f8_gemm(const acc950_f8_gemm_call* call);
 int64_t acc950_f8_gemm_workspace(const acc950_f8_gemm_call* call); /* (reads no memory but the call's) */
-#define ACC950_F8_VARIANT_ANY 0  /* 64x64 tiles, element by element: any strides and alignments */
+#define ACC950_F8_VARIANT_ANY 0  /* 64x64 tiles, element by element: any strides and alignments; fp32 sums throughout */
 #define ACC950_F8_VARIANT_TILE 1 /* + i: LDS tiles of 256x256, 128x128, 64x64, 64x64 (fewer stages) (i = 0 .. 3) on the e4m3 instruction; + 4: with
                                     * fp32 sums throughout (i > 0; 256x256 takes group_cols 128 only) */
 #define ACC950_F8_VARIANT_FEW 16 /* + i: kernels for few rows (i = 0, 1: 16 or 128 columns to a workgroup), B streamed into registers; + 2: with fp32 sums throughout */
@@ -152,7 +155,7 @@ int acc950_expert_plan_within(const acc950_expert_plan_call* call, int64_t works
 int64_t acc950_expert_plan_workspace(int64_t tokens, int64_t top_k, int64_t experts);
 
 /*
- * C[r, j] = (product as acc950_f8_gemm, group_cols 128) of A's row for sorted row r and the matrix of r's expert.  `rows` is the
+ * C[r, j] = (product as acc950_f8_gemm, its sums too; group_cols 128) of A's row for sorted row r and the matrix of r's expert.  `rows` is the
  * number of (token, slot) pairs; `order` and `offsets` are a plan's.  A's row is order[r] / top_k with gather = 1 (A by token) and
  * r with gather = 0.  B[e] starts at e * b_expert_stride, its scales at e * bs_expert_stride.  row_weights: NULL, or one
  * fp32 factor per pair (by pair, not by sorted row), applied before C is rounded.  Rows of C behind offsets[experts] are not written.
@@ -195,7 +198,10 @@ int acc950_expert_combine(const acc950_expert_combine_call* call);
  * A routed feed-forward layer: y[t] = sum over slots of weights[t, slot] * W2[e] * q(silu(W1[e] q(x[t])) * (W3[e] q(x[t]))), where q quantises rows
  * with power-of-two scales and e = ids[t, slot].  x and y: tokens x hidden of `type` F16 / BF16.  w13: (experts, 2, inner, hidden) e4m3 -- gate
  * and up --, scales (experts, 2, ceil(inner / 128), ceil(hidden / 128)); w2: (experts, hidden, inner), scales
- * (experts, ceil(hidden / 128), ceil(inner / 128)); all contiguous, w13 and w2 from 16-byte boundaries on.  Sums are fp32, rounded once, to `type`.
+ * (experts, ceil(hidden / 128), ceil(inner / 128)); all contiguous, w13 and w2 from 16-byte boundaries on.
+ * Numerics: up to 16 rows for each expert (tokens * top_k <= 16 * experts) all sums are fp32 and rounded once, to `type`.  With more, the sums of the down product, and for BF16 those of
+ * the gate and up product, are the e4m3 instruction's (see acc950_f8_gemm: about 1 in 5000 of the inner codes is its neighbour then); and for BF16 a token's rows, the terms of its
+ * weighted sum, are kept in 16 bits: fp16 with a power of two for each 32 or 64 columns, 2^-12 of a value beside the result's 2^-9.  The weighted sum itself is fp32.
  * `workspace` holds acc950_f8_expert_ffn_workspace bytes, 256-byte aligned;
  * acc950_f8_expert_ffn takes that on trust, acc950_f8_expert_ffn_within checks it.  It needs no clearing and may be used again by calls that follow each other on
  * a stream, but not by two that may run at the same time: steps' results and the counters that hand out tiles lie there.

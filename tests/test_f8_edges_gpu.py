@@ -360,3 +360,26 @@ def test_a_layer_with_few_rows_has_sums_in_fp32(acc, tokens, k, experts, hidden,
     moved = (got != want.to(got.dtype)).float().mean(dim=1)
     same = (moved < 0.02).float().mean()  # (of a token's results: those whose rounding the sums' last bits change, 2 * 2^-20 / 2^-11 and less)
     assert same >= 1 - max(0.05, 1.5 / tokens), (float(same), moved.tolist())
+
+
+# ---- what the sums hold ------------------------------------------------------------------------------------------------
+
+def test_products_whose_terms_cancel(acc):  # noqa: F811
+    """2^16 + 2^2 - 2^16: results in fp32, and the kernels with fp32 sums throughout whatever the result's type, hold what is left; other 16-bit results may be off by 2^-13 of the
+    largest of eight terms for each of them."""
+    import torch
+    f8 = torch.float8_e4m3fn
+    for m, n, k in ((1, 64, 128), (64, 128, 256), (300, 384, 512)):
+        a, w = torch.zeros(m, k), torch.ones(n, k)
+        a[:, 0], a[:, 1], a[:, 2] = 256, 2, -256
+        w[:, 0], w[:, 1], w[:, 2] = 256, 2, 256
+        blocks = k // 128
+        da, dw, sa, sw = a.to(f8).cuda(), w.to(f8).cuda(), torch.ones(m, blocks, device="cuda"), torch.ones(-(-n // 128), blocks, device="cuda")
+        for kind, variants in (("f32", [-1]), ("f16", [-1, 0, 6, 7, 8, 18, 19]), ("bf16", [-1, 0, 6, 7, 8, 18, 19])):
+            for variant in variants:
+                c = torch.empty((m, n), dtype=_dtype(kind), device="cuda")
+                acc.gemm_f8(da, sa, dw.t(), sw.t(), c, variant=variant)
+                if kind == "f32" or variant >= 0:
+                    assert (c == 4).all(), (m, kind, variant)
+                else:
+                    assert ((c.float() - 4).abs() <= 8 * 2.0 ** 16 * 2.0 ** -13).all()
