@@ -87,7 +87,7 @@ def quantize_f8(x, out=None, scale=None, *, group_rows=1, transpose=False, activ
     Groups of 128 run along q's last axis; ``group_rows`` (1, or 128 for a weight) rows share a scale.  ``transpose``: q is the
     transposed matrix.  ``activation``: "none", "relu", or "silu_mul" of x = [gate | up] (q is half as wide).  ``power_of_two``:
     scales are powers of two, so that only the codes are rounded.  An all-zero group has the scale 2^-126; an infinity or NaN makes its whole
-    group NaN.
+    group NaN, behind a ReLU too (a product's ReLU makes NaN 0).
 
     q (rows, cols) has rows that start on 16-byte boundaries unless ``out`` says otherwise; scale is (ceil(rows / group_rows), ceil(cols / 128)),
     laid out by blocks for single rows, as the product reads them.

@@ -37,7 +37,7 @@ extern "C" {
  * groups of 128 run along q's rows (its last axis) and group_rows (1 or 128) rows of q share a scale.
  *   s = max(largest |v| of the group / 448, 2^-126)   (power_of_two: the smallest power of two that is not below that)
  *   q = v * (1 / s), rounded to nearest even;  scale = s
- * An infinity or NaN makes its whole group stand for NaN.  q's elements are contiguous along its last axis.
+ * An infinity or NaN makes its whole group stand for NaN, behind a ReLU too (which keeps a NaN, unlike the product's).  q's elements are contiguous along its last axis.
  * scale[i, b] (i: group of rows, b: block) lies at i * s_row_stride + b * s_block_stride.  Activations go with transpose = 0.
  */
 typedef struct acc950_f8_quantize_call {
@@ -55,7 +55,7 @@ int acc950_f8_quantize(const acc950_f8_quantize_call* call);
 
 /*
  * C[i, j] = epilogue(sum over blocks b of a_scale[i, b] * b_scale[b, j / group_cols] * sum over k in b of A[i, k] * B[k, j]),
- * out_type F32 / F16 / BF16; epilogue ACC950_EPILOGUE_NONE or _RELU; group_cols 128 or 1.
+ * out_type F32 / F16 / BF16; epilogue ACC950_EPILOGUE_NONE or _RELU (v > 0 ? v : 0: a NaN gives 0, as everywhere in this library); group_cols 128 or 1.
  * Sums: blocks are added in fp32, always.  Inside a block, F32 results have fp32 sums throughout.  F16 and BF16 ones are left to the e4m3 matrix
  * instruction, twice as fast, which adds its products eight at a time and drops what lies below 2^-13 of the largest of them (2^16 + 2^2 gives 2^16): 2^-16 of a sum
  * of random terms, but 2^-13 of its largest terms where they cancel.  For fp32 sums take an F32 result, or one of the variants that name them below.

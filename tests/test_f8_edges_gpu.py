@@ -383,3 +383,27 @@ def test_products_whose_terms_cancel(acc):  # noqa: F811
                     assert (c == 4).all(), (m, kind, variant)
                 else:
                     assert ((c.float() - 4).abs() <= 8 * 2.0 ** 16 * 2.0 ** -13).all()
+
+
+def test_what_a_relu_makes_of_nan(acc):  # noqa: F811
+    """A product's ReLU is the library's (NaN gives 0, on every kernel); the one in front of quantising keeps a NaN, which makes its group NaN."""
+    import torch
+    for m, n, k in ((3, 130, 256), (70, 260, 300), (300, 520, 512), (200, 130, 9000)):
+        pitch = (k + 15) // 16 * 16
+        a, w = _codes(1, m, pitch)[:, :k], _codes(2, n, pitch)[:, :k]
+        a[1, 5] = float("nan")
+        blocks = -(-k // 128)
+        for kind in ("f32", "bf16"):
+            for variant in (-1, 0):
+                plain, relu = (torch.empty((m, n), dtype=_dtype(kind), device="cuda") for _ in range(2))
+                args = a.cuda(), _scales(3, m, blocks).cuda(), w.cuda().t(), _scales(4, -(-n // 128), blocks).cuda().t()
+                acc.gemm_f8(*args, plain, variant=variant)
+                acc.gemm_f8(*args, relu, epilogue=acc.EPILOGUE_RELU, variant=variant)
+                assert torch.isnan(plain[1]).all() and (relu[1] == 0).all()
+                assert torch.equal(relu[2:], torch.relu(plain[2:]))
+    x = _rand(1, 4, 256)
+    x[2, 200] = float("nan")
+    for group in (1, 128):
+        q, s = acc.quantize_f8(x.cuda(), activation="relu", group_rows=group)
+        v = q.float() * _spread(s, 4, 256, group)
+        assert torch.isnan(v[2, 128:]).all() and torch.isfinite(v[:, :128]).all()
