@@ -65,8 +65,9 @@ int acc950_f8_quantize(const acc950_f8_quantize_call* call);
  * are laid out anew in `workspace` first, if it holds them; otherwise every element is a load of its own.
  * `variant`: ACC950_VARIANT_AUTO, or ACC950_F8_VARIANT_*; one that does not take the problem returns ACC950_UNSUPPORTED.
  * K may go in slices whose fp32 sums meet in `workspace` (16-byte aligned, or NULL) and are added in their order by a second kernel: small results
- * with a long sum.  acc950_f8_gemm_workspace says how many bytes a call takes for all that; a smaller workspace is right too, or none (NULL).
- * k_slices: 0 = the library decides, n = at most n slices of a named tile variant (4 * M * (N rounded up to 4) bytes each).
+ * with a long sum.  acc950_f8_gemm_workspace says how many bytes a call takes for all that; a smaller workspace is right too with ACC950_VARIANT_AUTO, or none (NULL).
+ * k_slices: 0 = the library decides, n = at most n slices of a named tile variant (4 * M * (N rounded up to 4) bytes each), which is refused where the workspace
+ * does not hold them: a named variant is what the caller asked for, and what is said above of smaller workspaces goes for ACC950_VARIANT_AUTO.
  */
 typedef struct acc950_f8_gemm_call {
     int64_t out_type, M, N, K;
