@@ -38,13 +38,18 @@ struct F8TileConfig {
 __device__ __forceinline__ int f8_chunk(int row, int c) { return c ^ (row & 7); }
 
 // Straight from memory into LDS: lane l's 16 (4) bytes go to lds + 16 l (4 l); both base addresses are the same in all lanes.
+// A memory instruction may read a scalar register five instructions after a vector instruction has written it, no sooner (the compiler brings back spilled
+// ones with v_readlane, and does not look into inline assembly): the address is copied by the scalar unit, which waits by itself, and the copy stands where
+// m0 needs an instruction behind it anyway.
 __device__ __forceinline__ void fill_b128(unsigned lds, unsigned off, const void* base)
 {
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds), "v"(off), "s"(base) : "memory");
+    const void* at;
+    asm volatile("s_mov_b32 m0, %1\n\ts_mov_b64 %0, %3\n\tglobal_load_lds_dwordx4 %2, %0" : "=&s"(at) : "s"(lds), "v"(off), "s"(base) : "memory");
 }
 __device__ __forceinline__ void fill_b32(unsigned lds, unsigned off, const void* base)
 {
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, %2" ::"s"(lds), "v"(off), "s"(base) : "memory");
+    const void* at;
+    asm volatile("s_mov_b32 m0, %1\n\ts_mov_b64 %0, %3\n\tglobal_load_lds_dword %2, %0" : "=&s"(at) : "s"(lds), "v"(off), "s"(base) : "memory");
 }
 // All but the last N of the wave's fills have landed and its reads of LDS are done, in every wave.
 template <int N>
@@ -97,11 +102,11 @@ __device__ __forceinline__ i32x4 f8_cut16(i32x4 v, int inside)
 }
 
 // the low half of a product, and no more: with the addition behind it the compiler makes it a multiply-add of 64 bits, and keeps both halves
-// of the result in registers for as long as the one that is used
+// of the result in registers for as long as the one that is used.  (b goes through the scalar unit first, as in fill_b128: a vector instruction needs two between)
 __device__ __forceinline__ unsigned f8_mul32(unsigned a, unsigned b)
 {
-    unsigned d;
-    asm("v_mul_lo_u32 %0, %1, %2" : "=v"(d) : "v"(a), "s"(b));
+    unsigned d, copy;
+    asm("s_mov_b32 %1, %3\n\tv_mul_lo_u32 %0, %2, %1" : "=v"(d), "=&s"(copy) : "v"(a), "s"(b));
     return d;
 }
 

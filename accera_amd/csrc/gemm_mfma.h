@@ -314,12 +314,18 @@ struct OperandTile {
     }
 
     // Same for an address the register allocator may have put into vector registers although it is the same in every
-    // lane (scalar registers run short around the hand-laid loop): lane 0's copy is taken explicitly.
+    // lane (scalar registers run short around the hand-laid loop): lane 0's copy is taken explicitly.  A memory instruction may read a scalar register
+    // that a vector instruction wrote only five instructions later: the scalar unit, which waits by itself, copies it once more, where
+    // m0 needs an instruction behind it anyway.
     __device__ static __forceinline__ void direct_issue_uniform(unsigned lds_addr, unsigned lane_off, const char* sbase)
     {
         const unsigned long long a = (unsigned long long)sbase;
         const unsigned lo = __builtin_amdgcn_readfirstlane((unsigned)a), hi = __builtin_amdgcn_readfirstlane((unsigned)(a >> 32));
-        direct_issue(__builtin_amdgcn_readfirstlane(lds_addr), lane_off, (const char*)(((unsigned long long)hi << 32) | lo));
+        unsigned long long at;
+        asm volatile("s_mov_b32 m0, %1\n\ts_mov_b64 %0, %3\n\tglobal_load_lds_dwordx4 %2, %0"
+                     : "=&s"(at)
+                     : "s"(__builtin_amdgcn_readfirstlane(lds_addr)), "v"(lane_off), "s"(((unsigned long long)hi << 32) | lo)
+                     : "memory");
     }
 
     // ---- fragment read: 32 rows starting at row0, k-step ks (32 bytes of K) ----

@@ -109,9 +109,10 @@ __global__ void __launch_bounds__(512) mfma_traffic_kernel(const i32x4* src, con
                 const unsigned long long ga = (unsigned long long)g;
                 const unsigned lo = __builtin_amdgcn_readfirstlane((unsigned)ga), hi = __builtin_amdgcn_readfirstlane((unsigned)(ga >> 32));
                 const unsigned m0v = __builtin_amdgcn_readfirstlane(lds_base + stage + wave * 8192 + f * 1024);
-                asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2"
-                             :
-                             : "s"(m0v), "v"(lane_off), "s"((const char*)(((unsigned long long)hi << 32) | lo))
+                unsigned long long at; // (a copy by the scalar unit, which waits for the vector instruction in front; the fill would not)
+                asm volatile("s_mov_b32 m0, %1\n\ts_mov_b64 %0, %3\n\tglobal_load_lds_dwordx4 %2, %0"
+                             : "=&s"(at)
+                             : "s"(m0v), "v"(lane_off), "s"(((unsigned long long)hi << 32) | lo)
                              : "memory");
             }
         }
